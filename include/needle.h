@@ -273,6 +273,101 @@ int nd_attend_step_noalloc(const float *q, const void *k, const void *v, const f
                            const float *vs, int int8, int slots, const int *lo, const int *hi,
                            int B, int heads, int kv_heads, int qk, int vh, float *out, void *stream);
 
+/* ── drafted tokens: rotary positions, the cache's rows, a tree's attention,
+ * corrected logits. None has a counterpart in the reference, which decodes one
+ * token at a time. All run on the current device and `stream`, can be captured
+ * into a graph, keep nothing between calls, and refuse bad arguments with
+ * cudaErrorInvalidValue and a reason in nd_last_error(). Counts of zero do
+ * nothing. Indices in device memory (positions, sessions, token ids) are
+ * checked on the device as each entry says; nothing outside the given buffers
+ * is touched. ── */
+
+/* How rotation frequencies are stretched for contexts past the trained one.
+ * factor: the stretch. BY_PARTS: a pair that makes `fast` or more turns over
+ * `trained` positions keeps its frequency, one that makes `slow` or fewer is
+ * divided by factor, those between are blended linearly in the turns; mscale
+ * multiplies cos and sin (0: 1, or for BY_PARTS 0.1 ln(factor) + 1 when factor
+ * exceeds 1). */
+enum { ND_ROPE_PLAIN = 0, ND_ROPE_LINEAR = 1, ND_ROPE_BY_PARTS = 2 };
+typedef struct {
+  int kind;
+  double factor, trained, fast, slow;
+  float mscale;
+} NdRopeScaling;
+
+/* Rotary positions of x [M][ldx] into y [M][ldy] (y == x: in place; otherwise
+ * the two must not overlap): row i holds `heads` heads of head_dim floats side
+ * by side, at position pos[i] (device). The first rot_dim values of a head are
+ * rotated, the rest copied: pair j is (j, j + rot_dim / 2), or (2j, 2j + 1)
+ * when interleaved, turned by pos * theta^(-2j / rot_dim) (scaled as `scaling`
+ * says; NULL: plain); `inverse` turns back. Angles are formed and reduced in 64
+ * bits. Rows of negative position are left alone. rot_dim even, at most 256.
+ * Query and key heads that lie side by side in a projection's rows take one
+ * call. The engine's own rotation (v3/model.rs:378-413) is the half layout over
+ * the whole head. */
+int nd_rope(const float *x, int ldx, float *y, int ldy, const int *pos, int M, int heads, int head_dim,
+            int rot_dim, double theta, int interleaved, const NdRopeScaling *scaling, int inverse,
+            void *stream);
+
+/* Writes M rows of keys and values into KV rings of nd_attend_step's layout
+ * (kc [sessions][slots][kv_heads][qk], vc [..][vh], for int8 codes with scales
+ * ks, vs [sessions][slots][kv_heads]): row i, keys k + i * ldk and values v + i *
+ * ldv, goes to session sess[i] (NULL: i), slot pos[i] % slots. int8 quantises
+ * each head vector as nd_kv_quant does, bit for bit. A row of negative position
+ * or of a session outside 0..sessions-1 is skipped (a rejected or padding
+ * row). No two rows of a call may name the same session and slot, save one
+ * case: a session's rows stand one after another with ascending positions and
+ * pass the ring's length (a prompt longer than its ring), where the later
+ * rows win. Head widths up to 256, any strides. */
+int nd_kv_append(const float *k, int ldk, const float *v, int ldv, const int *sess, const int *pos, int M,
+                 int int8, int sessions, int slots, int kv_heads, int qk, int vh, void *kc, void *vc,
+                 float *ks, float *vs, void *stream);
+
+/* Reads rows back as floats (code * scale for int8): the reverse of
+ * nd_kv_append. Rows it would skip are left alone; k or v may be NULL; any rows
+ * may repeat. */
+int nd_kv_read(const void *kc, const void *vc, const float *ks, const float *vs, int int8, int sessions,
+               int slots, int kv_heads, int qk, int vh, const int *sess, const int *pos, int M, float *k,
+               int ldk, float *v, int ldv, void *stream);
+
+/* Attention of T drafted nodes per session over the session's ring and the
+ * draft itself. q: node t of session b at q + (b * T + t) * ldq, [heads][qk]
+ * floats; rings as for nd_attend_step, B sessions. Node (b, t) sees the ring
+ * positions lo[b * T + t] .. hi[b * T + t] (device, inclusive; empty when lo >
+ * hi; positions are logical, slot = position % slots, the newest `slots` of
+ * them count), and node j of its own draft when bit j % 32 of mask[(b * T + t) *
+ * ceil(T / 32) + j / 32] is set. The draft's keys and values tk, tv [B][T]
+ * [kv_heads][qk | vh] (int8: with scales tks, tvs) are a ring of T slots that
+ * nd_kv_append fills. mask NULL: a chain, node t sees nodes 0..t. tk and tv
+ * NULL: the ring only. out [B][T][heads][vh]; a node that sees nothing gets
+ * zeros, and what a node does not see never reaches its output, whatever it
+ * holds. heads / kv_heads may be any number; qk and vh multiples of 4 up to 128;
+ * T up to 4096. T = 1 is one decode step. Scores are scaled by 1 / sqrt(qk).
+ * Partial results of long rings use stream-ordered scratch. */
+int nd_attend_tree(const float *q, int ldq, const void *k, const void *v, const float *ks, const float *vs,
+                   int int8, int slots, const int *lo, const int *hi, const void *tk, const void *tv,
+                   const float *tks, const float *tvs, const uint32_t *mask, int B, int T, int heads,
+                   int kv_heads, int qk, int vh, float *out, void *stream);
+
+/* Corrects logits [rows][ld] into out [rows][ldo] (out == logits: in place) and
+ * picks each row's first maximum into picks [rows] (may be NULL). In order, for
+ * row r: a token that occurs in hist[hist_off[r] .. hist_off[r + 1]) is divided
+ * by repetition[r] when positive, else multiplied; one that occurs c > 0 times
+ * from hist[gen_from[r]] on (NULL: in all of it) loses c * frequency[r] +
+ * presence[r]; the biases of bias_ids[bias_off[r] .. bias_off[r + 1]) are
+ * added, in list order where an id repeats; a token whose bit (id % 32 of
+ * mask[r * mask_ld + id / 32]) is clear becomes `masked` (the grammar mask of
+ * needle_tokenizer_tool_mask uses -1e9; -INFINITY removes it from any
+ * softmax). All arrays are device memory. hist, bias_ids and mask may each be
+ * NULL: no token seen (the penalties then do nothing), no bias, no mask; so may
+ * each penalty. Ids outside 0..vocab-1 are ignored. A
+ * NaN is never picked; a row of -INFINITY or NaN alone picks 0. */
+int nd_logits_adjust(const float *logits, int ld, int rows, int vocab, float *out, int ldo, const int *hist,
+                     const int *hist_off, const int *gen_from, const float *repetition, const float *presence,
+                     const float *frequency, const int *bias_ids, const float *bias_vals,
+                     const int *bias_off, const uint32_t *mask, int mask_ld, float masked, uint32_t *picks,
+                     void *stream);
+
 /* Returns the cudaError_t of the last nd_* failure on this thread as text. */
 const char *nd_last_error(void);
 

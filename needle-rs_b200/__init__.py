@@ -149,6 +149,14 @@ def lib() -> C.CDLL:
         "nd_kv_quant": (C.c_int, [vp, C.c_int, C.c_int, vp, vp, vp]),
         "nd_attend_step": (C.c_int, [vp, vp, vp, vp, vp, C.c_int, C.c_int, vp, vp, C.c_int, C.c_int,
                                      C.c_int, C.c_int, C.c_int, vp, vp]),
+        "nd_rope": (C.c_int, [vp, C.c_int, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_double, C.c_int,
+                              vp, C.c_int, vp]),
+        "nd_kv_append": (C.c_int, [vp, C.c_int, vp, C.c_int, vp, vp] + [C.c_int] * 7 + [vp] * 5),
+        "nd_kv_read": (C.c_int, [vp] * 4 + [C.c_int] * 6 + [vp, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp]),
+        "nd_attend_tree": (C.c_int, [vp, C.c_int] + [vp] * 4 + [C.c_int, C.c_int] + [vp] * 7 + [C.c_int] * 6 +
+                           [vp, vp]),
+        "nd_logits_adjust": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, C.c_int] + [vp] * 10 +
+                             [C.c_int, C.c_float, vp, vp]),
         "nd_last_error": (C.c_char_p, []),
     }
     for name, (res, args) in sig.items():
@@ -511,3 +519,83 @@ def attend_step(q_ptr, k_ptr, v_ptr, ks_ptr, vs_ptr, int8, slots, lo_ptr, hi_ptr
                 qk, vh, out_ptr, stream=None):
     _check(lib().nd_attend_step(q_ptr, k_ptr, v_ptr, ks_ptr, vs_ptr, int(int8), slots, lo_ptr, hi_ptr, B,
                                 heads, kv_heads, qk, vh, out_ptr, stream), "nd_attend_step")
+
+
+# ------------------------------------------------------------ drafted tokens
+class RopeScaling(C.Structure):
+    """Stretched rotation frequencies (NdRopeScaling in needle.h): kind "plain",
+    "linear" or "by_parts"; mscale 0 takes the kind's own factor."""
+
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("trained", C.c_double), ("fast", C.c_double),
+                ("slow", C.c_double), ("mscale", C.c_float)]
+    KINDS = ("plain", "linear", "by_parts")
+
+    def __init__(self, kind="plain", factor=1.0, trained=0.0, fast=32.0, slow=1.0, mscale=0.0):
+        if kind not in self.KINDS:
+            raise NeedleError(f"RopeScaling: unknown kind {kind!r}")
+        super().__init__(self.KINDS.index(kind), factor, trained, fast, slow, mscale)
+
+
+def rope(x_ptr, ldx, y_ptr, ldy, pos_ptr, M, heads, head_dim, rot_dim=None, theta=10000.0, interleaved=False,
+         scaling=None, inverse=False, stream=None):
+    """Rotary positions of M rows of heads; y_ptr == x_ptr works in place."""
+    _check(lib().nd_rope(x_ptr, ldx, y_ptr, ldy, pos_ptr, M, heads, head_dim,
+                         head_dim if rot_dim is None else rot_dim, theta, interleaved,
+                         None if scaling is None else C.byref(scaling), inverse, stream), "nd_rope")
+
+
+def kv_append(k_ptr, ldk, v_ptr, ldv, sess_ptr, pos_ptr, M, int8, sessions, slots, kv_heads, qk, vh, kc_ptr, vc_ptr,
+              ks_ptr=None, vs_ptr=None, stream=None):
+    """Writes M rows of keys and values to rings, quantised for int8."""
+    _check(lib().nd_kv_append(k_ptr, ldk, v_ptr, ldv, sess_ptr, pos_ptr, M, int8, sessions, slots, kv_heads, qk, vh,
+                              kc_ptr, vc_ptr, ks_ptr, vs_ptr, stream), "nd_kv_append")
+
+
+def kv_read(kc_ptr, vc_ptr, ks_ptr, vs_ptr, int8, sessions, slots, kv_heads, qk, vh, sess_ptr, pos_ptr, M, k_ptr,
+            ldk, v_ptr, ldv, stream=None):
+    """Reads M rows of keys and values back from rings as floats."""
+    _check(lib().nd_kv_read(kc_ptr, vc_ptr, ks_ptr, vs_ptr, int8, sessions, slots, kv_heads, qk, vh, sess_ptr,
+                            pos_ptr, M, k_ptr, ldk, v_ptr, ldv, stream), "nd_kv_read")
+
+
+def tree_mask(parents) -> np.ndarray:
+    """The mask of a draft given every node's parent (-1: none; a parent comes
+    before its children): node t sees itself and its ancestors. [T][ceil(T /
+    32)] uint32 words for attend_tree, one session."""
+    T = len(parents)
+    m = np.zeros((T, (T + 31) // 32), np.uint32)
+    for t, p in enumerate(parents):
+        if not -1 <= p < t:
+            raise NeedleError(f"tree_mask: node {t} has parent {p}")
+        if p >= 0:
+            m[t] = m[p]
+        m[t, t // 32] |= np.uint32(1 << (t % 32))
+    return m
+
+
+def attend_tree(q_ptr, ldq, k_ptr, v_ptr, ks_ptr, vs_ptr, int8, slots, lo_ptr, hi_ptr, tk_ptr, tv_ptr, tks_ptr,
+                tvs_ptr, mask_ptr, B, T, heads, kv_heads, qk, vh, out_ptr, stream=None):
+    """Attention of T drafted nodes per session over rings and the draft."""
+    _check(lib().nd_attend_tree(q_ptr, ldq, k_ptr, v_ptr, ks_ptr, vs_ptr, int8, slots, lo_ptr, hi_ptr, tk_ptr,
+                                tv_ptr, tks_ptr, tvs_ptr, mask_ptr, B, T, heads, kv_heads, qk, vh, out_ptr, stream),
+           "nd_attend_tree")
+
+
+def pack_mask(allowed) -> np.ndarray:
+    """Token bits for logits_adjust from truth values, or from a grammar mask of
+    needle_tokenizer_tool_mask (0 allowed, negative forbidden): [..][ceil(n /
+    32)] uint32 words."""
+    a = np.asarray(allowed)
+    a = a.astype(bool) if a.dtype.kind in "bui" else a >= 0
+    pad = -a.shape[-1] % 32
+    a = np.concatenate([a, np.zeros(a.shape[:-1] + (pad,), bool)], -1)
+    return np.ascontiguousarray(np.packbits(a, axis=-1, bitorder="little")).view(np.uint32)
+
+
+def logits_adjust(logits_ptr, ld, rows, vocab, out_ptr, ldo, hist_ptr=None, hist_off_ptr=None, gen_from_ptr=None,
+                  repetition_ptr=None, presence_ptr=None, frequency_ptr=None, bias_ids_ptr=None, bias_vals_ptr=None,
+                  bias_off_ptr=None, mask_ptr=None, mask_ld=0, masked=float("-inf"), picks_ptr=None, stream=None):
+    """Penalties, biases and a token mask on rows of logits, and their greedy picks."""
+    _check(lib().nd_logits_adjust(logits_ptr, ld, rows, vocab, out_ptr, ldo, hist_ptr, hist_off_ptr, gen_from_ptr,
+                                  repetition_ptr, presence_ptr, frequency_ptr, bias_ids_ptr, bias_vals_ptr,
+                                  bias_off_ptr, mask_ptr, mask_ld, masked, picks_ptr, stream), "nd_logits_adjust")

@@ -5,6 +5,7 @@
 // results are NULL on failure, boolean results false, sizes 0.
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <fstream>
@@ -1099,6 +1100,129 @@ int nd_attend_step(const float* q, const void* k, const void* v, const float* ks
   e = nb::launch_attend_step(q, k, v, ks, vs, int8, slots, lo, hi, B, heads, kv_heads, qk, vh, ns, part, out, st);
   cudaError_t f = cudaFreeAsync(part, st);
   return nd_status(e != cudaSuccess ? e : f);
+}
+
+// A refused nd_* call: the reason in nd_last_error().
+static int nd_refuse(const char* why) {
+  nb::nd_record_error(cudaErrorInvalidValue, why);
+  return (int)cudaErrorInvalidValue;
+}
+static bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+
+int nd_rope(const float* x, int ldx, float* y, int ldy, const int* pos, int M, int heads, int head_dim, int rot_dim,
+            double theta, int interleaved, const NdRopeScaling* scaling, int inverse, void* stream) {
+  if (M < 0) return nd_refuse("nd_rope: negative row count");
+  if (M == 0) return 0;
+  if (!x || !y || !pos) return nd_refuse("nd_rope: null pointer");
+  if (heads <= 0 || head_dim <= 0 || (long)heads * head_dim > (1 << 24))
+    return nd_refuse("nd_rope: heads and head_dim must be positive, their product at most 2^24");
+  if (rot_dim <= 0 || rot_dim % 2 || rot_dim > head_dim || rot_dim > nb::ROPE_MAX_ROT)
+    return nd_refuse("nd_rope: rot_dim must be even, in 2..min(head_dim, 256)");
+  if (ldx < heads * head_dim || ldy < heads * head_dim)
+    return nd_refuse("nd_rope: a row stride is shorter than heads * head_dim");
+  if (x == y && ldx != ldy) return nd_refuse("nd_rope: in place, both strides must agree");
+  if (!(theta > 0.0) || !(theta <= 1e30)) return nd_refuse("nd_rope: theta must be in (0, 1e30]");
+  NdRopeScaling s = {ND_ROPE_PLAIN, 1.0, 0.0, 0.0, 0.0, 0.f};
+  if (scaling) s = *scaling;
+  if (s.kind < ND_ROPE_PLAIN || s.kind > ND_ROPE_BY_PARTS) return nd_refuse("nd_rope: unknown scaling kind");
+  if (s.kind != ND_ROPE_PLAIN && (!(s.factor > 0.0) || !(s.factor <= 1e30)))
+    return nd_refuse("nd_rope: the scaling factor must be in (0, 1e30]");
+  if (s.kind == ND_ROPE_BY_PARTS && (!(s.trained > 0.0) || !(s.slow >= 0.0) || !(s.fast > s.slow)))
+    return nd_refuse("nd_rope: scaling by parts needs trained > 0 and fast > slow >= 0");
+  float m = s.mscale;
+  if (m == 0.f) m = s.kind == ND_ROPE_BY_PARTS && s.factor > 1.0 ? (float)(0.1 * std::log(s.factor) + 1.0) : 1.f;
+  return nd_status(nb::launch_rope(x, ldx, y, ldy, pos, M, heads, head_dim, rot_dim, theta, interleaved != 0, s.kind,
+                                   s.factor, s.trained, s.fast, s.slow, m, inverse != 0, (cudaStream_t)stream));
+}
+
+int nd_kv_append(const float* k, int ldk, const float* v, int ldv, const int* sess, const int* pos, int M, int int8,
+                 int sessions, int slots, int kv_heads, int qk, int vh, void* kc, void* vc, float* ks, float* vs,
+                 void* stream) {
+  if (M < 0) return nd_refuse("nd_kv_append: negative row count");
+  if (M == 0) return 0;
+  if (!k || !v || !pos || !kc || !vc || (int8 && (!ks || !vs))) return nd_refuse("nd_kv_append: null pointer");
+  if (kv_heads <= 0 || kv_heads > 512 || qk <= 0 || qk > 256 || vh <= 0 || vh > 256)
+    return nd_refuse("nd_kv_append: kv_heads must be in 1..512, head widths in 1..256");
+  if (sessions <= 0 || slots <= 0) return nd_refuse("nd_kv_append: sessions and slots must be positive");
+  if (!sess && M > sessions) return nd_refuse("nd_kv_append: without session indices, at most one row per session");
+  if (ldk < kv_heads * qk || ldv < kv_heads * vh)
+    return nd_refuse("nd_kv_append: a row stride is shorter than the row");
+  return nd_status(nb::launch_kv_append(k, ldk, v, ldv, sess, pos, M, int8, sessions, slots, kv_heads, qk, vh, kc, vc,
+                                        ks, vs, (cudaStream_t)stream));
+}
+
+int nd_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, int int8, int sessions, int slots,
+               int kv_heads, int qk, int vh, const int* sess, const int* pos, int M, float* k, int ldk, float* v,
+               int ldv, void* stream) {
+  if (M < 0) return nd_refuse("nd_kv_read: negative row count");
+  if (M == 0) return 0;
+  if (!k && !v) return nd_refuse("nd_kv_read: neither keys nor values asked for");
+  if (!pos || (k && (!kc || (int8 && !ks))) || (v && (!vc || (int8 && !vs))))
+    return nd_refuse("nd_kv_read: null pointer");
+  if (kv_heads <= 0 || kv_heads > 512 || qk <= 0 || qk > 256 || vh <= 0 || vh > 256)
+    return nd_refuse("nd_kv_read: kv_heads must be in 1..512, head widths in 1..256");
+  if (sessions <= 0 || slots <= 0) return nd_refuse("nd_kv_read: sessions and slots must be positive");
+  if (!sess && M > sessions) return nd_refuse("nd_kv_read: without session indices, at most one row per session");
+  if ((k && ldk < kv_heads * qk) || (v && ldv < kv_heads * vh))
+    return nd_refuse("nd_kv_read: a row stride is shorter than the row");
+  return nd_status(nb::launch_kv_read(kc, vc, ks, vs, int8, sessions, slots, kv_heads, qk, vh, sess, pos, M, k, ldk,
+                                      v, ldv, (cudaStream_t)stream));
+}
+
+int nd_attend_tree(const float* q, int ldq, const void* k, const void* v, const float* ks, const float* vs, int int8,
+                   int slots, const int* lo, const int* hi, const void* tk, const void* tv, const float* tks,
+                   const float* tvs, const uint32_t* mask, int B, int T, int heads, int kv_heads, int qk, int vh,
+                   float* out, void* stream) {
+  if (B < 0 || T < 0) return nd_refuse("nd_attend_tree: negative count");
+  if (B == 0 || T == 0) return 0;
+  if (!q || !k || !v || !lo || !hi || !out || (int8 && (!ks || !vs)))
+    return nd_refuse("nd_attend_tree: null pointer");
+  if (!tk != !tv || (tk && int8 && (!tks || !tvs)))
+    return nd_refuse("nd_attend_tree: a draft needs keys, values and, for int8, both scales");
+  if (mask && !tk) return nd_refuse("nd_attend_tree: a mask without drafted keys and values");
+  if (kv_heads <= 0 || kv_heads > 512 || heads <= 0 || heads % kv_heads)
+    return nd_refuse("nd_attend_tree: kv_heads must be in 1..512 and divide heads");
+  if (qk <= 0 || vh <= 0 || qk % 4 || vh % 4 || qk > 128 || vh > 128)
+    return nd_refuse("nd_attend_tree: head widths must be multiples of 4, at most 128");
+  if (T > 4096 || slots <= 0 || slots > (1 << 30))
+    return nd_refuse("nd_attend_tree: T must be at most 4096, slots in 1..2^30");
+  if ((long)B * T > (1l << 30) / heads) return nd_refuse("nd_attend_tree: B * T * heads above 2^30");
+  if ((long)ldq < (long)heads * qk) return nd_refuse("nd_attend_tree: ldq is shorter than heads * qk");
+  if (!aligned(k, 4) || !aligned(v, 4) || !aligned(tk, 4) || !aligned(tv, 4))
+    return nd_refuse("nd_attend_tree: cache pointers must be 4-byte aligned");
+  cudaStream_t st = (cudaStream_t)stream;
+  const int ns = nb::tree_nsplit(B, T, heads, kv_heads, qk, vh, slots);
+  float* part = nullptr;
+  if (ns > 1) {
+    cudaError_t e = scratch_alloc((void**)&part, nb::tree_part_floats(B, T, heads, vh, ns) * 4, st);
+    if (e != cudaSuccess) return nd_status(e);
+  }
+  cudaError_t e = nb::launch_attend_tree(q, ldq, k, v, ks, vs, int8, slots, lo, hi, tk, tv, tks, tvs, mask, B, T,
+                                         heads, kv_heads, qk, vh, ns, part, out, st);
+  if (part) {
+    const cudaError_t f = cudaFreeAsync(part, st);
+    if (e == cudaSuccess) e = f;
+  }
+  return nd_status(e);
+}
+
+int nd_logits_adjust(const float* logits, int ld, int rows, int vocab, float* out, int ldo, const int* hist,
+                     const int* hist_off, const int* gen_from, const float* repetition, const float* presence,
+                     const float* frequency, const int* bias_ids, const float* bias_vals, const int* bias_off,
+                     const uint32_t* mask, int mask_ld, float masked, uint32_t* picks, void* stream) {
+  if (rows < 0) return nd_refuse("nd_logits_adjust: negative row count");
+  if (rows == 0) return 0;
+  if (!logits || !out) return nd_refuse("nd_logits_adjust: null pointer");
+  if (vocab <= 0 || vocab > (1 << 30)) return nd_refuse("nd_logits_adjust: vocab must be in 1..2^30");
+  if (ld < vocab || ldo < vocab) return nd_refuse("nd_logits_adjust: a row stride is shorter than vocab");
+  if (logits == out && ld != ldo) return nd_refuse("nd_logits_adjust: in place, both strides must agree");
+  if (hist && !hist_off) return nd_refuse("nd_logits_adjust: a history needs its row offsets");
+  if (bias_ids && (!bias_vals || !bias_off))
+    return nd_refuse("nd_logits_adjust: biases need ids, values and row offsets");
+  if (mask && (long)mask_ld * 32 < vocab) return nd_refuse("nd_logits_adjust: mask_ld is shorter than vocab / 32 words");
+  return nd_status(nb::launch_logits_adjust(logits, ld, rows, vocab, out, ldo, hist, hist_off, gen_from, repetition,
+                                            presence, frequency, bias_ids, bias_vals, bias_off, mask, mask_ld, masked,
+                                            picks, (cudaStream_t)stream));
 }
 
 const char* nd_last_error(void) { return g_nd_err.c_str(); }

@@ -223,4 +223,32 @@ cudaError_t launch_attend_step(const float* q, const void* k, const void* v, con
                                int B, int heads, int kvh, int qk, int vh, int nsplit, float* part,
                                float* out, cudaStream_t st);
 
+// Widest rotated part of a head that launch_rope takes.
+constexpr int ROPE_MAX_ROT = 256;
+// Standalone rotary positions (rope_kernels.cu). kind 0 plain, 1 linear, 2 by
+// parts; y may be x. Rows of negative position are left alone.
+cudaError_t launch_rope(const float* x, int ldx, float* y, int ldy, const int* pos, int M, int heads, int dim, int rot,
+                        double theta, bool interleaved, int kind, double factor, double trained, double fast,
+                        double slow, float mscale, bool inverse, cudaStream_t st);
+// Rows written to and read from rings of nd_attend_step's layout (kv_kernels.cu).
+cudaError_t launch_kv_append(const float* k, int ldk, const float* v, int ldv, const int* sess, const int* pos, int M,
+                             int int8, int sessions, int slots, int kvh, int qk, int vh, void* kc, void* vc, float* ks,
+                             float* vs, cudaStream_t st);
+cudaError_t launch_kv_read(const void* kc, const void* vc, const float* ks, const float* vs, int int8, int sessions,
+                           int slots, int kvh, int qk, int vh, const int* sess, const int* pos, int M, float* k,
+                           int ldk, float* v, int ldv, cudaStream_t st);
+// Attention of drafted nodes (tree_kernels.cu); `part` is scratch of
+// tree_part_floats(..) floats (none for one split).
+int tree_nsplit(int B, int T, int heads, int kvh, int qk, int vh, int slots);
+size_t tree_part_floats(int B, int T, int heads, int vh, int nsplit);
+cudaError_t launch_attend_tree(const float* q, int ldq, const void* k, const void* v, const float* ks, const float* vs,
+                               int int8, int slots, const int* lo, const int* hi, const void* tk, const void* tv,
+                               const float* tks, const float* tvs, const uint32_t* mask, int B, int T, int heads,
+                               int kvh, int qk, int vh, int nsplit, float* part, float* out, cudaStream_t st);
+// Corrections and greedy pick of logit rows (logit_kernels.cu).
+cudaError_t launch_logits_adjust(const float* x, int ldx, int rows, int vocab, float* y, int ldy, const int* hist,
+                                 const int* hist_off, const int* gen_from, const float* rep, const float* pres,
+                                 const float* freq, const int* bias_ids, const float* bias_vals, const int* bias_off,
+                                 const uint32_t* mask, int mask_ld, float masked, uint32_t* picks, cudaStream_t st);
+
 }  // namespace nb

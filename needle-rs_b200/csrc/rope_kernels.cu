@@ -1,0 +1,137 @@
+// Rotary positions of any layout: nd_rope. The forward's own rotation (half
+// layout over the whole head, table built at load, v3/model.rs:378-413) stays
+// inside qkv_post; this is the standalone form for projections a caller keeps,
+// with the pair layouts, partial heads and context scalings other callers use.
+#include <cmath>
+
+#include "kernels.hpp"
+#include "fastdiv.hpp"
+
+namespace nb {
+
+// Frequencies in turns per position, in 64 bits: pair i of a token at position
+// p is rotated by frac(p * turns[i]) turns. The product and its reduction stay
+// in 64 bits because a 32-bit angle p * w has an absolute error of p * w *
+// 2^-24, 0.06 rad at position 2^20; the reduced fraction (at most half a turn)
+// is then exact enough in 32.
+struct RopeFreqs {
+  double turns[ROPE_MAX_ROT / 2];
+  float m;    // factor of cos and sin
+  float sgn;  // -1 rotates back
+};
+
+// One block: `tok` tokens. Its threads first form the tokens' cosines and sines
+// in shared memory (once per token and pair, shared by all heads), then stream
+// the rows. An item is the piece of a head that one thread rotates:
+//   VEC, half layout: float4 at pairs 4j.. and the float4 half a rotation on;
+//   VEC, interleaved: one float4 (two pairs);
+//   scalar: one pair.
+// Items past the rotated part copy (nothing when y is x).
+// Bytes bound it: 8 per value; see launch_rope for the figures.
+template <bool VEC, bool INTER>
+__global__ void __launch_bounds__(256) rope_kernel(const float* x, long ldx, float* y, long ldy,
+                                                   const int* __restrict__ pos, int M, int heads, int dim, int rot,
+                                                   int tok, FastDiv per_head, FastDiv per_tok, int copy,
+                                                   const __grid_constant__ RopeFreqs F) {
+  extern __shared__ __align__(16) float cs[];  // [tok][rot / 2] cosines, then sines
+  const int half = rot >> 1;
+  float* sn = cs + tok * half;
+  const int t0 = blockIdx.x * tok, nt = min(tok, M - t0);
+  for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
+    const int t = i / half, j = i - t * half;
+    const double turn = (double)pos[t0 + t] * F.turns[j];
+    float s, c;
+    sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
+    cs[i] = c * F.m;
+    sn[i] = s * F.m * F.sgn;
+  }
+  __syncthreads();
+  const int total = nt * (int)per_tok.d;
+  // Pieces of a head: rotating ones first, then copies.
+  const int nrot = VEC ? (INTER ? rot >> 2 : half >> 2) : half;
+#pragma unroll 2
+  for (int it = threadIdx.x; it < total; it += blockDim.x) {
+    const int t = per_tok.div(it), r = it - t * (int)per_tok.d;
+    const int h = per_head.div(r), j = r - h * (int)per_head.d;
+    if (pos[t0 + t] < 0) continue;  // padding row: left as it is
+    const float* xr = x + (size_t)(t0 + t) * ldx + (size_t)h * dim;
+    float* yr = y + (size_t)(t0 + t) * ldy + (size_t)h * dim;
+    const float *c = cs + t * half, *s = sn + t * half;
+    if (j < nrot) {
+      if (VEC && !INTER) {
+        const float4 a = *reinterpret_cast<const float4*>(xr + 4 * j);
+        const float4 b = *reinterpret_cast<const float4*>(xr + half + 4 * j);
+        const float4 cc = *reinterpret_cast<const float4*>(c + 4 * j), ss = *reinterpret_cast<const float4*>(s + 4 * j);
+        *reinterpret_cast<float4*>(yr + 4 * j) = make_float4(a.x * cc.x - b.x * ss.x, a.y * cc.y - b.y * ss.y,
+                                                             a.z * cc.z - b.z * ss.z, a.w * cc.w - b.w * ss.w);
+        *reinterpret_cast<float4*>(yr + half + 4 * j) = make_float4(a.x * ss.x + b.x * cc.x, a.y * ss.y + b.y * cc.y,
+                                                                    a.z * ss.z + b.z * cc.z, a.w * ss.w + b.w * cc.w);
+      } else if (VEC) {
+        const float4 a = *reinterpret_cast<const float4*>(xr + 4 * j);
+        const float2 cc = *reinterpret_cast<const float2*>(c + 2 * j), ss = *reinterpret_cast<const float2*>(s + 2 * j);
+        *reinterpret_cast<float4*>(yr + 4 * j) =
+            make_float4(a.x * cc.x - a.y * ss.x, a.x * ss.x + a.y * cc.x, a.z * cc.y - a.w * ss.y,
+                        a.z * ss.y + a.w * cc.y);
+      } else {
+        const int p0 = INTER ? 2 * j : j, p1 = INTER ? 2 * j + 1 : j + half;
+        const float a = xr[p0], b = xr[p1];
+        yr[p0] = a * c[j] - b * s[j];
+        yr[p1] = a * s[j] + b * c[j];
+      }
+    } else if (copy) {
+      const int e = VEC ? rot + 4 * (j - nrot) : rot + (j - nrot);
+      if (VEC)
+        *reinterpret_cast<float4*>(yr + e) = *reinterpret_cast<const float4*>(xr + e);
+      else
+        yr[e] = xr[e];
+    }
+  }
+}
+
+cudaError_t launch_rope(const float* x, int ldx, float* y, int ldy, const int* pos, int M, int heads, int dim, int rot,
+                        double theta, bool interleaved, int kind, double factor, double trained, double fast,
+                        double slow, float mscale, bool inverse, cudaStream_t st) {
+  if (M <= 0) return cudaSuccess;
+  RopeFreqs F;
+  const double two_pi = 6.283185307179586476925;
+  for (int i = 0; i < rot / 2; ++i) {
+    double f = std::pow(theta, -2.0 * i / rot) / two_pi;
+    if (kind == 1) {
+      f /= factor;
+    } else if (kind == 2) {
+      // Turns the pair makes over the trained context: above `fast` it keeps
+      // its frequency, below `slow` it is stretched, in between a blend.
+      const double r = trained * f;
+      const double keep = std::fmin(1.0, std::fmax(0.0, (r - slow) / (fast - slow)));
+      f = f * keep + f / factor * (1.0 - keep);
+    }
+    F.turns[i] = f;
+  }
+  F.m = mscale;
+  F.sgn = inverse ? -1.0f : 1.0f;
+  const int half = rot / 2;
+  const bool vec = dim % 4 == 0 && rot % 4 == 0 && (interleaved || half % 4 == 0) && ldx % 4 == 0 && ldy % 4 == 0 &&
+                   ((uintptr_t)x | (uintptr_t)y) % 16 == 0;
+  const int copy = x == y ? 0 : 1;
+  const int nrot = vec ? (interleaved ? rot / 4 : half / 4) : half;
+  const int nhead = nrot + (copy ? (dim - rot) / (vec ? 4 : 1) : 0);
+  const long items = (long)heads * nhead;
+  // Tokens per block: one while that leaves SMs idle, else enough for about
+  // 1024 items (four per thread) and at most 8, so that cosines and sines are
+  // formed by most threads at once.
+  int tok = 1;
+  while (tok < 8 && (long)M > 592L * tok && items * tok < 1024) tok *= 2;
+  const size_t smem = (size_t)tok * rot * sizeof(float);
+  const dim3 grid((M + tok - 1) / tok);
+  const FastDiv ph(nhead), pt((uint32_t)items);
+#define NB_ROPE(V, I) \
+  rope_kernel<V, I><<<grid, 256, smem, st>>>(x, ldx, y, ldy, pos, M, heads, dim, rot, tok, ph, pt, copy, F)
+  if (vec && interleaved) NB_ROPE(true, true);
+  else if (vec) NB_ROPE(true, false);
+  else if (interleaved) NB_ROPE(false, true);
+  else NB_ROPE(false, false);
+#undef NB_ROPE
+  return cudaGetLastError();
+}
+
+}  // namespace nb
