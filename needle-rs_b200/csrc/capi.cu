@@ -1191,14 +1191,15 @@ int nd_attend_tree(const float* q, int ldq, const void* k, const void* v, const 
   if (!aligned(k, 4) || !aligned(v, 4) || !aligned(tk, 4) || !aligned(tv, 4))
     return nd_refuse("nd_attend_tree: cache pointers must be 4-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
-  const int ns = nb::tree_nsplit(B, T, heads, kv_heads, qk, vh, slots);
+  const nb::TreePlan plan = nb::tree_plan(k, v, tk, tv, out, int8, B, T, heads, kv_heads, qk, vh, slots);
+  const int ns = plan.nsplit;
   float* part = nullptr;
   if (ns > 1) {
     cudaError_t e = scratch_alloc((void**)&part, nb::tree_part_floats(B, T, heads, vh, ns) * 4, st);
     if (e != cudaSuccess) return nd_status(e);
   }
   cudaError_t e = nb::launch_attend_tree(q, ldq, k, v, ks, vs, int8, slots, lo, hi, tk, tv, tks, tvs, mask, B, T,
-                                         heads, kv_heads, qk, vh, ns, part, out, st);
+                                         heads, kv_heads, qk, vh, plan, part, out, st);
   if (part) {
     const cudaError_t f = cudaFreeAsync(part, st);
     if (e == cudaSuccess) e = f;

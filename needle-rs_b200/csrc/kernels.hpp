@@ -239,12 +239,19 @@ cudaError_t launch_kv_read(const void* kc, const void* vc, const float* ks, cons
                            int ldk, float* v, int ldv, cudaStream_t st);
 // Attention of drafted nodes (tree_kernels.cu); `part` is scratch of
 // tree_part_floats(..) floats (none for one split).
-int tree_nsplit(int B, int T, int heads, int kvh, int qk, int vh, int slots);
+struct TreePlan {
+  bool umma;   // tcgen05 form (tree_umma.cu)
+  int piece;   // bytes of a copy the cache's alignment allows
+  int nsplit;  // position splits
+};
+TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv, const float* out, int int8, int B,
+                   int T, int heads, int kvh, int qk, int vh, int slots);
 size_t tree_part_floats(int B, int T, int heads, int vh, int nsplit);
 cudaError_t launch_attend_tree(const float* q, int ldq, const void* k, const void* v, const float* ks, const float* vs,
                                int int8, int slots, const int* lo, const int* hi, const void* tk, const void* tv,
                                const float* tks, const float* tvs, const uint32_t* mask, int B, int T, int heads,
-                               int kvh, int qk, int vh, int nsplit, float* part, float* out, cudaStream_t st);
+                               int kvh, int qk, int vh, const TreePlan& plan, float* part, float* out,
+                               cudaStream_t st);
 // Corrections and greedy pick of logit rows (logit_kernels.cu).
 cudaError_t launch_logits_adjust(const float* x, int ldx, int rows, int vocab, float* y, int ldy, const int* hist,
                                  const int* hist_off, const int* gen_from, const float* rep, const float* pres,

@@ -16,9 +16,9 @@
 // and remainders. Sums, max and the outputs are f32.
 #include <algorithm>
 
-#include "fastdiv.hpp"
 #include "kernels.hpp"
 #include "launch_util.hpp"
+#include "tree.cuh"
 
 namespace nb {
 namespace {
@@ -33,24 +33,6 @@ __device__ __forceinline__ int tree_dim(int n, int col) {
 
 constexpr int TREE_WARPS = 4;
 constexpr int TREE_THREADS = TREE_WARPS * 32;
-
-struct TreeArgs {
-  const float* q;
-  long ldq;
-  const char *k, *v;       // ring [B][slots][kvh][qk | vh]
-  const float *ks, *vs;    // [B][slots][kvh]
-  const char *tk, *tv;     // draft [B][T][kvh][qk | vh]
-  const float *tks, *tvs;  // [B][T][kvh]
-  const int *lo, *hi;      // [B][T]
-  const uint32_t* mask;    // [B][T][words] or null: a chain
-  int slots, T, heads, kvh, rep, qk, vh, words;
-  int drafted;             // T when the draft's keys are given, else 0
-  int nsplit;
-  float scale;             // log2(e) / sqrt(qk)
-  FastDiv by_rep;
-  float* out;              // [B][T][heads][vh]
-  float* part;             // [B][kvh][nsplit][T * rep][vh + 2] when nsplit > 1
-};
 
 __device__ __forceinline__ void mma_h(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -71,12 +53,6 @@ __device__ __forceinline__ void ldm4t(uint32_t (&r)[4], const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"((unsigned)__cvta_generic_to_shared(p)));
-}
-// 2^x, relative error about 2^-22; arguments here are <= 0.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ uint32_t h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -717,20 +693,8 @@ cudaError_t launch_tree(TreeArgs A, int B, int piece, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int R = A.T * A.rep, tiles = (R + MT * 16 - 1) / (MT * 16);
   for (int b0 = 0; b0 < B; b0 += 65535) {
-    TreeArgs C = A;
     const int n = std::min(65535, B - b0);
-    const size_t ring = (size_t)b0 * A.slots * A.kvh, draft = (size_t)b0 * A.T * A.kvh;
-    C.q += (size_t)b0 * A.T * A.ldq;
-    C.k += ring * A.qk * TT::ES, C.v += ring * A.vh * TT::ES;
-    if (A.drafted) C.tk += draft * A.qk * TT::ES, C.tv += draft * A.vh * TT::ES;
-    if (I8) {
-      C.ks += ring, C.vs += ring;
-      if (A.drafted) C.tks += draft, C.tvs += draft;
-    }
-    C.lo += (size_t)b0 * A.T, C.hi += (size_t)b0 * A.T;
-    if (A.mask) C.mask += (size_t)b0 * A.T * A.words;
-    C.out += (size_t)b0 * A.T * A.heads * A.vh;
-    if (A.part) C.part += (size_t)b0 * A.kvh * A.nsplit * R * (A.vh + 2);
+    const TreeArgs C = tree_sessions(A, b0, TT::ES);
     kern<<<dim3((unsigned)tiles * A.kvh * A.nsplit, n), TREE_THREADS, smem, st>>>(C, piece);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -742,13 +706,25 @@ int tree_tile_rows(int R, int qk, int vh) { return R <= 16 || qk > 64 || vh > 64
 
 }  // namespace
 
-// Position splits of a call: enough blocks for about four a SM, each split at
-// least 8 blocks of 32 positions.
-int tree_nsplit(int B, int T, int heads, int kvh, int qk, int vh, int slots) {
-  const int R = T * (heads / kvh), tr = tree_tile_rows(R, qk, vh);
+// How a call runs: on tcgen05 or mma.sync, and over how many position splits.
+// mma.sync: enough blocks for about four a SM, each split at least 8 blocks of
+// 32 positions.
+TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv, const float* out, int int8, int B,
+                   int T, int heads, int kvh, int qk, int vh, int slots) {
+  const int es = int8 ? 1 : 4, R = T * (heads / kvh);
+  auto al16 = [](const void* p) { return (uintptr_t)p % 16 == 0; };
+  TreePlan P;
+  P.piece = qk * es % 16 == 0 && vh * es % 16 == 0 && al16(k) && al16(v) && al16(tk) && al16(tv) ? 16 : 4;
+  P.umma = al16(out) && tree_umma_takes(int8, R, qk, vh, P.piece);
+  if (P.umma) {
+    P.nsplit = tree_umma_nsplit(int8, B, R, kvh, qk, vh, slots + (tk ? T : 0));
+    return P;
+  }
+  const int tr = tree_tile_rows(R, qk, vh);
   const long ctas = (long)B * kvh * ((R + tr - 1) / tr);
   const long want = (592 + ctas - 1) / ctas, most = std::max(1, (slots + 255) / 256);
-  return (int)std::max(1l, std::min(std::min(want, most), 256l));
+  P.nsplit = (int)std::max(1l, std::min(std::min(want, most), 256l));
+  return P;
 }
 
 size_t tree_part_floats(int B, int T, int heads, int vh, int nsplit) {
@@ -758,7 +734,8 @@ size_t tree_part_floats(int B, int T, int heads, int vh, int nsplit) {
 cudaError_t launch_attend_tree(const float* q, int ldq, const void* k, const void* v, const float* ks, const float* vs,
                                int int8, int slots, const int* lo, const int* hi, const void* tk, const void* tv,
                                const float* tks, const float* tvs, const uint32_t* mask, int B, int T, int heads,
-                               int kvh, int qk, int vh, int nsplit, float* part, float* out, cudaStream_t st) {
+                               int kvh, int qk, int vh, const TreePlan& plan, float* part, float* out,
+                               cudaStream_t st) {
   if (B <= 0 || T <= 0) return cudaSuccess;
   TreeArgs A;
   A.q = q, A.ldq = ldq;
@@ -766,26 +743,25 @@ cudaError_t launch_attend_tree(const float* q, int ldq, const void* k, const voi
   A.tk = (const char*)tk, A.tv = (const char*)tv, A.tks = tks, A.tvs = tvs;
   A.lo = lo, A.hi = hi, A.mask = mask;
   A.slots = slots, A.T = T, A.heads = heads, A.kvh = kvh, A.rep = heads / kvh, A.qk = qk, A.vh = vh;
-  A.words = (T + 31) / 32, A.drafted = tk ? T : 0, A.nsplit = nsplit;
+  A.words = (T + 31) / 32, A.drafted = tk ? T : 0, A.nsplit = plan.nsplit;
   A.scale = (float)(1.4426950408889634 / sqrt((double)qk));
   A.by_rep = FastDiv(A.rep);
   A.out = out, A.part = part;
-  const int es = int8 ? 1 : 4;
-  auto al16 = [](const void* p) { return (uintptr_t)p % 16 == 0; };
-  const int piece = qk * es % 16 == 0 && vh * es % 16 == 0 && al16(k) && al16(v) && al16(tk) && al16(tv) ? 16 : 4;
+  const int piece = plan.piece;
   const int R = T * A.rep;
   cudaError_t e;
   const bool one = tree_tile_rows(R, qk, vh) == 16;
 #define NB_TREE(Q, V, M) e = int8 ? launch_tree<true, Q, V, M>(A, B, piece, st) : launch_tree<false, Q, V, M>(A, B, piece, st)
-  if (qk > 64 || vh > 64) NB_TREE(128, 128, 1);
+  if (plan.umma) e = launch_tree_umma(A, int8, B, st);
+  else if (qk > 64 || vh > 64) NB_TREE(128, 128, 1);
   else if (qk > 48 && one) NB_TREE(64, 64, 1);
   else if (qk > 48) NB_TREE(64, 64, 2);
   else if (one) NB_TREE(48, 64, 1);
   else NB_TREE(48, 64, 2);
 #undef NB_TREE
-  if (e != cudaSuccess || nsplit == 1) return e;
+  if (e != cudaSuccess || plan.nsplit == 1) return e;
   const long rows = (long)B * T * heads;
-  tree_join_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(part, (int)rows, R, T, heads, kvh, A.rep, vh, nsplit,
+  tree_join_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(part, (int)rows, R, T, heads, kvh, A.rep, vh, plan.nsplit,
                                                                out);
   return cudaGetLastError();
 }
