@@ -22,24 +22,30 @@ struct RopeFreqs {
 
 // One block: `tok` tokens. Its threads first form the tokens' cosines and sines
 // in shared memory (once per token and pair, shared by all heads), then stream
-// the rows. An item is the piece of a head that one thread rotates:
+// the rows, ROPE_FLIGHT items a thread loaded before the first is stored. An
+// item is the piece of a head that one thread takes:
 //   VEC, half layout: float4 at pairs 4j.. and the float4 half a rotation on;
 //   VEC, interleaved: one float4 (two pairs);
 //   scalar: one pair.
-// Items past the rotated part copy (nothing when y is x).
+// Items past the rotated part copy (there are none when y is x).
 // Bytes bound it: 8 per value; see launch_rope for the figures.
+constexpr int ROPE_FLIGHT = 4;
+
 template <bool VEC, bool INTER>
 __global__ void __launch_bounds__(256) rope_kernel(const float* x, long ldx, float* y, long ldy,
-                                                   const int* __restrict__ pos, int M, int heads, int dim, int rot,
-                                                   int tok, FastDiv per_head, FastDiv per_tok, int copy,
+                                                   const int* __restrict__ pos, int M, int dim, int rot, int tok,
+                                                   FastDiv per_head, FastDiv per_tok,
                                                    const __grid_constant__ RopeFreqs F) {
-  extern __shared__ __align__(16) float cs[];  // [tok][rot / 2] cosines, then sines
+  extern __shared__ __align__(16) float cs[];  // [tok][rot / 2] cosines, then sines; then the positions
   const int half = rot >> 1;
   float* sn = cs + tok * half;
+  int* at = reinterpret_cast<int*>(sn + tok * half);
   const int t0 = blockIdx.x * tok, nt = min(tok, M - t0);
   for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
     const int t = i / half, j = i - t * half;
-    const double turn = (double)pos[t0 + t] * F.turns[j];
+    const int p = pos[t0 + t];
+    if (j == 0) at[t] = p;
+    const double turn = (double)p * F.turns[j];
     float s, c;
     sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
     cs[i] = c * F.m;
@@ -49,41 +55,59 @@ __global__ void __launch_bounds__(256) rope_kernel(const float* x, long ldx, flo
   const int total = nt * (int)per_tok.d;
   // Pieces of a head: rotating ones first, then copies.
   const int nrot = VEC ? (INTER ? rot >> 2 : half >> 2) : half;
-#pragma unroll 2
-  for (int it = threadIdx.x; it < total; it += blockDim.x) {
-    const int t = per_tok.div(it), r = it - t * (int)per_tok.d;
-    const int h = per_head.div(r), j = r - h * (int)per_head.d;
-    if (pos[t0 + t] < 0) continue;  // padding row: left as it is
-    const float* xr = x + (size_t)(t0 + t) * ldx + (size_t)h * dim;
-    float* yr = y + (size_t)(t0 + t) * ldy + (size_t)h * dim;
-    const float *c = cs + t * half, *s = sn + t * half;
-    if (j < nrot) {
-      if (VEC && !INTER) {
-        const float4 a = *reinterpret_cast<const float4*>(xr + 4 * j);
-        const float4 b = *reinterpret_cast<const float4*>(xr + half + 4 * j);
-        const float4 cc = *reinterpret_cast<const float4*>(c + 4 * j), ss = *reinterpret_cast<const float4*>(s + 4 * j);
-        *reinterpret_cast<float4*>(yr + 4 * j) = make_float4(a.x * cc.x - b.x * ss.x, a.y * cc.y - b.y * ss.y,
-                                                             a.z * cc.z - b.z * ss.z, a.w * cc.w - b.w * ss.w);
-        *reinterpret_cast<float4*>(yr + half + 4 * j) = make_float4(a.x * ss.x + b.x * cc.x, a.y * ss.y + b.y * cc.y,
-                                                                    a.z * ss.z + b.z * cc.z, a.w * ss.w + b.w * cc.w);
-      } else if (VEC) {
-        const float4 a = *reinterpret_cast<const float4*>(xr + 4 * j);
-        const float2 cc = *reinterpret_cast<const float2*>(c + 2 * j), ss = *reinterpret_cast<const float2*>(s + 2 * j);
-        *reinterpret_cast<float4*>(yr + 4 * j) =
-            make_float4(a.x * cc.x - a.y * ss.x, a.x * ss.x + a.y * cc.x, a.z * cc.y - a.w * ss.y,
-                        a.z * ss.y + a.w * cc.y);
+  for (int base = threadIdx.x; base < total; base += blockDim.x * ROPE_FLIGHT) {
+    float4 a[ROPE_FLIGHT], b[ROPE_FLIGHT];
+    float* to[ROPE_FLIGHT];
+    int sc[ROPE_FLIGHT];  // where the piece's cosines lie, -1 for a copy
+#pragma unroll
+    for (int u = 0; u < ROPE_FLIGHT; ++u) {
+      const int it = base + u * blockDim.x;
+      to[u] = nullptr;
+      if (it >= total) continue;
+      const int t = per_tok.div(it), r = it - t * (int)per_tok.d;
+      if (at[t] < 0) continue;  // padding row: left as it is
+      const int h = per_head.div(r), j = r - h * (int)per_head.d;
+      const size_t from = (size_t)(t0 + t) * ldx + (size_t)h * dim;
+      to[u] = y + (size_t)(t0 + t) * ldy + (size_t)h * dim;
+      const bool turn = j < nrot;
+      // offset of the piece in the head
+      const int e = VEC ? (turn ? 4 * j : rot + 4 * (j - nrot)) : (turn ? (INTER ? 2 * j : j) : rot + (j - nrot));
+      sc[u] = turn ? t * half + (VEC ? (INTER ? 2 * j : 4 * j) : j) : -1;
+      to[u] += e;
+      if (VEC) {
+        a[u] = *reinterpret_cast<const float4*>(x + from + e);
+        if (!INTER && turn) b[u] = *reinterpret_cast<const float4*>(x + from + e + half);
       } else {
-        const int p0 = INTER ? 2 * j : j, p1 = INTER ? 2 * j + 1 : j + half;
-        const float a = xr[p0], b = xr[p1];
-        yr[p0] = a * c[j] - b * s[j];
-        yr[p1] = a * s[j] + b * c[j];
+        a[u].x = x[from + e];
+        if (turn) b[u].x = x[from + e + (INTER ? 1 : half)];
       }
-    } else if (copy) {
-      const int e = VEC ? rot + 4 * (j - nrot) : rot + (j - nrot);
-      if (VEC)
-        *reinterpret_cast<float4*>(yr + e) = *reinterpret_cast<const float4*>(xr + e);
-      else
-        yr[e] = xr[e];
+    }
+#pragma unroll
+    for (int u = 0; u < ROPE_FLIGHT; ++u) {
+      if (!to[u]) continue;
+      if (sc[u] < 0) {
+        if (VEC) *reinterpret_cast<float4*>(to[u]) = a[u];
+        else *to[u] = a[u].x;
+        continue;
+      }
+      const float *c = cs + sc[u], *s = sn + sc[u];
+      if (VEC && !INTER) {
+        const float4 cc = *reinterpret_cast<const float4*>(c), ss = *reinterpret_cast<const float4*>(s);
+        *reinterpret_cast<float4*>(to[u]) = make_float4(a[u].x * cc.x - b[u].x * ss.x, a[u].y * cc.y - b[u].y * ss.y,
+                                                        a[u].z * cc.z - b[u].z * ss.z, a[u].w * cc.w - b[u].w * ss.w);
+        *reinterpret_cast<float4*>(to[u] + half) =
+            make_float4(a[u].x * ss.x + b[u].x * cc.x, a[u].y * ss.y + b[u].y * cc.y, a[u].z * ss.z + b[u].z * cc.z,
+                        a[u].w * ss.w + b[u].w * cc.w);
+      } else if (VEC) {
+        const float2 cc = *reinterpret_cast<const float2*>(c), ss = *reinterpret_cast<const float2*>(s);
+        *reinterpret_cast<float4*>(to[u]) =
+            make_float4(a[u].x * cc.x - a[u].y * ss.x, a[u].x * ss.x + a[u].y * cc.x, a[u].z * cc.y - a[u].w * ss.y,
+                        a[u].z * ss.y + a[u].w * cc.y);
+      } else {
+        const float p = a[u].x, q = b[u].x;
+        to[u][0] = p * c[0] - q * s[0];
+        to[u][INTER ? 1 : half] = p * s[0] + q * c[0];
+      }
     }
   }
 }
@@ -121,11 +145,11 @@ cudaError_t launch_rope(const float* x, int ldx, float* y, int ldy, const int* p
   // formed by most threads at once.
   int tok = 1;
   while (tok < 8 && (long)M > 592L * tok && items * tok < 1024) tok *= 2;
-  const size_t smem = (size_t)tok * rot * sizeof(float);
+  const size_t smem = (size_t)tok * (rot + 1) * sizeof(float);
   const dim3 grid((M + tok - 1) / tok);
   const FastDiv ph(nhead), pt((uint32_t)items);
 #define NB_ROPE(V, I) \
-  rope_kernel<V, I><<<grid, 256, smem, st>>>(x, ldx, y, ldy, pos, M, heads, dim, rot, tok, ph, pt, copy, F)
+  rope_kernel<V, I><<<grid, 256, smem, st>>>(x, ldx, y, ldy, pos, M, dim, rot, tok, ph, pt, F)
   if (vec && interleaved) NB_ROPE(true, true);
   else if (vec) NB_ROPE(true, false);
   else if (interleaved) NB_ROPE(false, true);

@@ -3,7 +3,7 @@
 //
 //   S = Q K^T,  P = 2^(S * scales - max),  O += P V
 //
-// per block of BN positions: S and O lie in tensor memory (TMEM), a softmax
+// per step of 64 positions: S and O lie in tensor memory (TMEM), a softmax
 // warpgroup holds one row a thread, P returns to TMEM in S's place as the A
 // operand of the second product. f32 accuracy from f16 operands: the query and
 // P are f16 high parts and remainders (22 bits; int8 codes are f16 values
@@ -13,13 +13,16 @@
 // and truncation costs only what the sum already holds. For the same reason O
 // is drained into f32 registers after every block.
 //
-// Warps: W softmax warpgroups (block i belongs to warpgroup i % W, each its
-// own running max, sum and output, merged at the end) and four producer warps
-// that read the ring and the draft, widen them to f16 and lay them down in the
-// 128-byte swizzled form the MMA reads: keys as they lie, values transposed
-// eight positions at a time in registers. With W = 1 two blocks share an SM, so one's
-// softmax runs under the other's MMAs; 128-wide heads need the shared memory
-// of a whole SM and W = 2. One thread of a softmax warpgroup issues its MMAs.
+// Warps: W softmax warpgroups (step i belongs to warpgroup i % W, each with its
+// own running max, sum and output, merged at the end), and for each another one of
+//   a key warp and two value warps, which read the ring and the draft, widen
+//   them to f16 and lay them down in the 128-byte swizzled form the MMA reads
+//   (keys as they lie, values transposed eight positions at a time in
+//   registers; the key warp also forms the steps' scales), and
+//   an MMA warp, which issues every product as soon as its operands stand: a
+//   warp that issues MMAs is held for as long as they run.
+// With W = 1 two blocks share an SM and hide each other's latencies; 128-wide
+// heads need the shared memory of a whole SM and W = 2.
 //
 // Every wait is bounded as in umma_gemm.cu.
 #include <algorithm>
@@ -32,32 +35,33 @@
 namespace nb {
 namespace {
 
-template <bool I8_, int QS_, int VP_, int W_, int BN_, int NST_>
+template <bool I8_, int QS_, int VP_, int W_, int NST_>
 struct TreeUmma {
   static constexpr bool I8 = I8_;
   static constexpr int QS = QS_;    // k16 steps of the key product
   static constexpr int VP = VP_;    // value width held (64 or 128)
-  static constexpr int W = W_, BN = BN_, NST = NST_;
+  static constexpr int W = W_, NST = NST_;
+  static constexpr int BN = 64;                   // positions of a stage, and of a step of the softmax
   static constexpr int KA = (QS * 16 + 63) / 64;  // 64-wide swizzle atoms of a key row
   static constexpr int PARTS = I8 ? 1 : 2;        // high part, remainder
-  static constexpr int Q_TILE = KA * 128 * 128, K_TILE = KA * BN * 128, V_TILE = BN / 64 * VP * 128;
+  static constexpr int Q_TILE = KA * 128 * 128, K_TILE = KA * BN * 128, V_TILE = VP * 128;
   static constexpr int STAGE = PARTS * (K_TILE + V_TILE);
-  static constexpr int THREADS = W * 128 + 128, CTAS = W == 1 ? 2 : 1;
-  // Registers a thread: the launch's, a softmax thread's, a producer's; the
-  // warpgroups' shares add up to the launch's.
-  static constexpr int REG_ALL = W == 1 ? 128 : 168, REG_SOFT = W == 1 ? 168 : 208, REG_PROD = 88;
-  static_assert(W * REG_SOFT + REG_PROD == (W + 1) * REG_ALL, "register shares");
-  static constexpr int S_COLS = BN, WG_COLS = BN + VP;  // TMEM columns of a warpgroup: S (then P), O
+  static constexpr int THREADS = 2 * W * 128, CTAS = W == 1 ? 2 : 1;
+  // Registers a thread: the launch's, a softmax thread's, the other warpgroup's;
+  // the warpgroups' shares add up to the launch's.
+  static constexpr int REG_ALL = 128, REG_SOFT = W == 1 ? (I8 ? 184 : 176) : 192, REG_PROD = 256 - REG_SOFT;
+  static constexpr int WG_COLS = 2 * BN + VP;     // TMEM columns of a warpgroup: two of S (then P), O
   static constexpr int TMEM = W * WG_COLS <= 128 ? 128 : W * WG_COLS <= 256 ? 256 : 512;
-  static constexpr size_t META = NST * (size_t)(BN * 8 + BN / 8 + 16) + 128 * 4 + 512 + 2 * 4 * 64 * 4;
+  static constexpr size_t META = NST * (size_t)(BN * 8 + 16 + 16) + 128 * 4 + 512;
   static constexpr size_t SMEM = 1024 + 2 * (size_t)Q_TILE + NST * (size_t)STAGE + META;
 };
 
 __device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]));
 }
+// As tmem_wait_ld, but ordinary loads may move across it.
+__device__ __forceinline__ void tmem_landed() { asm volatile("tcgen05.wait::ld.sync.aligned;"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // kind::f16: f32 accumulate, f16 operands, both K-major, M = 128.
@@ -79,6 +83,23 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(tree_idesc<N>()), "r"(accum));
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(t));
+}
+// One lane of a converged warp, in a form the compiler knows to be uniform.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
 }
 
 typedef unsigned long long f32x2;
@@ -143,6 +164,11 @@ struct TreePlace {
     int s = slot0 + (v - drafted);
     if (s >= slots) s -= slots;
     return ring + (size_t)s * kvh;
+  }
+  // Whether positions v .. v + n - 1 are ring places one after another.
+  __device__ __forceinline__ bool plain(int v, int n) const {
+    const int s = slot0 + (v - drafted);
+    return v >= drafted && v + n <= total && (s + n <= slots || s >= slots);
   }
 };
 
@@ -227,21 +253,23 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
   unsigned char *qhi = sm, *qlo = sm + C::Q_TILE, *stages = sm + 2 * C::Q_TILE;
   float* col_k = reinterpret_cast<float*>(stages + (size_t)NST * C::STAGE);  // [NST][BN] key scales
   float* col_v = col_k + NST * BN;                                          // [NST][BN] value scales times 2^(140 - e)
-  uint32_t* odd = reinterpret_cast<uint32_t*>(col_v + NST * BN);            // [NST][NC] columns to keep out
-  int* expo = reinterpret_cast<int*>(odd + NST * NC);                       // [NST][2] e, least exponent so far
+  uint32_t* odd = reinterpret_cast<uint32_t*>(col_v + NST * BN);            // [NST][NC] columns to keep out (f32: of keys, of values)
+  int* expo = reinterpret_cast<int*>(odd + NST * 4);                       // [NST][2] e, least exponent so far
   float* row_q = reinterpret_cast<float*>(expo + 2 * NST);                  // [128] score scale of a row
-  float* wmax = row_q + 128;                                                // [2][4][64] producers' maxima
-  uint64_t* full = reinterpret_cast<uint64_t*>(wmax + 2 * 4 * 64);
+  uint64_t* full = reinterpret_cast<uint64_t*>(row_q + 128);
   uint64_t* empty = full + NST;
-  uint64_t* s_full = empty + NST;   // [W] S of the warpgroup's block
-  uint64_t* o_full = s_full + W;    // [W] O of the warpgroup's block
-  uint64_t* drain = o_full + W;     // [W] every MMA of the warpgroup
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + W);
+  uint64_t* s_full = empty + NST;   // [W][2] S of the warpgroup's sub-block
+  uint64_t* o_full = s_full + 2 * W;  // [W] O of the warpgroup's sub-block
+  uint64_t* p_full = o_full + W;    // [W] P of the warpgroup's step, one arrival a warp with rows
+  uint64_t* q_full = p_full + W;    // the queries
+  uint64_t* drain = q_full + 1;     // every MMA
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile uint32_t* abort = tmem_slot + 1;
   int* range = reinterpret_cast<int*>(tmem_slot + 2);    // [2]
   uint32_t* slow = reinterpret_cast<uint32_t*>(range + 2);  // [4] rows for tree_slow_row
+  int* vmax = reinterpret_cast<int*>(slow + 4);             // [2][4] the value warps' exponents
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int b = blockIdx.y;
   int bx = blockIdx.x;
   const int z = bx % A.nsplit;
@@ -252,14 +280,17 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
 
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
-      mbar_init(&full[s], 128);  // the producers
+      mbar_init(&full[s], 96);   // the key and value warps
       mbar_init(&empty[s], 1);   // one tcgen05.commit
     }
     for (int w = 0; w < W; ++w) {
-      mbar_init(&s_full[w], 1);
+      mbar_init(&s_full[2 * w], 1);
+      mbar_init(&s_full[2 * w + 1], 1);
       mbar_init(&o_full[w], 1);
-      mbar_init(&drain[w], 1);
+      mbar_init(&p_full[w], (rows + 31) / 32);
     }
+    mbar_init(q_full, 128);
+    mbar_init(drain, 1);
     *abort = 0;
     range[0] = 0x7fffffff, range[1] = -1;
     slow[0] = slow[1] = slow[2] = slow[3] = 0;
@@ -270,9 +301,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
                  "r"((uint32_t)C::TMEM));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // Zeros where the copies never write: dims past the heads' widths, rows past the tile's.
-  for (int i = tid * 16; i < 2 * C::Q_TILE + NST * C::STAGE; i += C::THREADS * 16)
-    *reinterpret_cast<uint4*>(sm + i) = make_uint4(0, 0, 0, 0);
+  // Zeros where nothing is ever written: dims past the heads' widths.
+  if (A.qk != QS * 16 || A.vh != VP)
+    for (int i = tid * 16; i < 2 * C::Q_TILE + NST * C::STAGE; i += C::THREADS * 16)
+      *reinterpret_cast<uint4*>(sm + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
   for (int n = n0 + tid; n <= n1; n += C::THREADS) {
     const int h = A.hi[(size_t)b * A.T + n];
@@ -283,44 +315,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       atomicMax(&range[1], h);
     }
   }
-  // Queries: two threads a row, each half of its dims; scaled by the power of
-  // two that brings the row's max into [2^13, 2^14).
-  if (tid < 256) {
-    const int r = tid >> 1, half = tid & 1;
-    const bool in = r < rows;
-    const int rr = r0 + (in ? r : 0), n = A.by_rep.div(rr), h = kh * A.rep + rr - n * A.rep;
-    const float* q = A.q + ((size_t)b * A.T + n) * A.ldq + (size_t)h * A.qk;
-    constexpr int HC = QS;  // 8-dim chunks of a half row
-    float mx = 0.f;
-    for (int c = 0; c < HC; ++c)
-      for (int i = 0; i < 8; ++i) {
-        const int d = (half * HC + c) * 8 + i;
-        if (in && d < A.qk) mx = fmaxf(mx, fabsf(__ldg(q + d)));
-      }
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    const int ef = (int)(__float_as_uint(mx) >> 23);
-    const int ex = ef == 0 || ef >= 255 ? 0 : min(140 - ef, 126);
-    const float by = __uint_as_float((uint32_t)(127 + ex) << 23);
-    for (int c = 0; c < HC; ++c) {
-      const int ch = half * HC + c;  // 16-byte chunk of the row: atom ch / 8
-      uint32_t hh[4], ll[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = ch * 8 + 2 * i;
-        const float x = in && d < A.qk ? __ldg(q + d) * by : 0.f, y = in && d + 1 < A.qk ? __ldg(q + d + 1) * by : 0.f;
-        halves(x, y, &hh[i], &ll[i]);
-      }
-      const int at = (ch >> 3) * 128 * 128 + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-      *reinterpret_cast<uint4*>(qhi + at) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
-      *reinterpret_cast<uint4*>(qlo + at) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
-    }
-    if (half == 0) row_q[r] = A.scale * __uint_as_float((uint32_t)(127 - ex) << 23);
-  }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int base = range[1] >= 0 ? range[0] : 0;
   const int n_ring = range[1] >= 0 ? (int)min((long)range[1] - base + 1, (long)A.slots) : 0;
   TreePlace P;
@@ -349,7 +348,42 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
     // ------------------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFT));
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + wg * C::WG_COLS, o_at = s_at + C::S_COLS;
+    const uint32_t s_at = tmem + wg * C::WG_COLS, o_at = s_at + 128;
+    // ---- queries: a row a thread of the first warpgroup, scaled by the power
+    // of two that brings the row's max into [2^13, 2^14)
+    if (wg == 0) {
+      const float* q = A.q + node_at * A.ldq + (size_t)head * A.qk;
+      float x[QS * 16];
+      if (mine && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+#pragma unroll
+        for (int c = 0; c < QS * 4; ++c) {
+          const float4 f = c * 4 < A.qk ? __ldg(reinterpret_cast<const float4*>(q) + c) : make_float4(0, 0, 0, 0);
+          x[4 * c] = f.x, x[4 * c + 1] = f.y, x[4 * c + 2] = f.z, x[4 * c + 3] = f.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < QS * 16; ++i) x[i] = mine && i < A.qk ? __ldg(q + i) : 0.f;
+      }
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < QS * 16; ++i) mx = fmaxf(mx, fabsf(x[i]));
+      const int ef = (int)(__float_as_uint(mx) >> 23);
+      const int ex = ef == 0 || ef >= 255 ? 0 : min(140 - ef, 126);
+      const float by = __uint_as_float((uint32_t)(127 + ex) << 23);
+#pragma unroll
+      for (int c = 0; c < 2 * QS; ++c) {
+        uint32_t hh[4], ll[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) halves(x[8 * c + 2 * i] * by, x[8 * c + 2 * i + 1] * by, &hh[i], &ll[i]);
+        const int at = (c >> 3) * 128 * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(qhi + at) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
+        *reinterpret_cast<uint4*>(qlo + at) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
+      }
+      row_q[r] = A.scale * __uint_as_float((uint32_t)(127 - ex) << 23);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(q_full);
+    }
+    if (W == 2) asm volatile("bar.sync 3, 256;" ::: "memory");
     const float qs = row_q[r];
     // Positions every row of the warp sees without a look at the mask.
     int full0 = A.drafted + start, full1 = A.drafted + min(start + cnt, n_ring);
@@ -363,109 +397,101 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
     bool is_slow = false, ok = true;
 #pragma unroll
     for (int d = 0; d < VP / 2; ++d) o[d] = pk(0.f, 0.f);
-    const bool issuer = (tid & 127) == 0;
-
-    auto issue_qk = [&](int i) {  // S of block i
-      const int st = i % NST;
-      if (!mbar_wait(&full[st], (uint32_t)(i / NST) & 1u, abort, werr)) return;
-      tc_fence_after();
-      unsigned char* kt = stages + (size_t)st * C::STAGE;
-      const uint64_t dqh = sw128_desc(qhi), dql = sw128_desc(qlo), dk = sw128_desc(kt);
-      uint32_t acc = 0;
-      auto steps = [&](uint64_t dq, uint64_t dkk) {
-#pragma unroll
-        for (int k = 0; k < QS; ++k) {
-          mma_ss<BN>(s_at, dq + (uint64_t)((k >> 2) * (128 * 128 >> 4) + (k & 3) * 2),
-                     dkk + (uint64_t)((k >> 2) * (BN * 128 >> 4) + (k & 3) * 2), acc);
-          acc = 1;
-        }
-      };
-      steps(dql, dk);
-      if (!I8) steps(dqh, dk + (uint64_t)(C::K_TILE >> 4));
-      steps(dqh, dk);
-      umma_commit(&s_full[wg]);
-    };
-    auto issue_pv = [&](int i) {  // O of block i
-      const int st = i % NST;
-      unsigned char* vt = stages + (size_t)st * C::STAGE + C::PARTS * C::K_TILE;
-      const uint64_t dv = sw128_desc(vt);
-      uint32_t acc = 0;
-      auto steps = [&](uint32_t a, uint64_t dvv) {
-#pragma unroll
-        for (int k = 0; k < BN / 16; ++k) {
-          mma_ts<VP>(o_at, a + k * 16, dvv + (uint64_t)((k >> 2) * (VP * 128 >> 4) + (k & 3) * 2),
-                     acc);
-          acc = 1;
-        }
-      };
-      steps(s_at + 8, dv);
-      if (!I8) steps(s_at, dv + (uint64_t)(C::V_TILE >> 4));
-      steps(s_at, dv);
-      umma_commit(&o_full[wg]);
-      umma_commit(&empty[st]);
-    };
-    if (issuer && wg < nblk) issue_qk(wg);
-    __syncwarp();
+    // Step jj of the warpgroup takes stage i = jj W + wg. Warps whose rows are
+    // all padding take no part.
+    const int nj = (warp & 3) * 32 < rows && nblk > wg ? (nblk - wg + W - 1) / W : 0;
 
     int e_old = 14, it = 0;
     int low = 255;
-    for (int i = wg; i < nblk; i += W, ++it) {
-      const int st = i % NST;
-      if (ok && !mbar_wait(&s_full[wg], (uint32_t)it & 1u, abort, werr)) ok = false;
-      if (ok && !mbar_wait(&full[st], (uint32_t)(i / NST) & 1u, abort, werr)) ok = false;
+    for (int jj = 0; jj < nj; ++jj, ++it) {
+      const int i = jj * W + wg, st = i % NST;
+      if (ok && !mbar_wait_asleep(&s_full[2 * wg + (jj & 1)], (uint32_t)(jj >> 1) & 1u, abort, werr)) ok = false;
+      if (ok && !mbar_wait_asleep(&full[st], (uint32_t)(i / NST) & 1u, abort, werr)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
         const int v0 = (blk0 + i) * BN;
+        const uint32_t s_now = s_at + lanes + (jj & 1) * BN;
         const float4* k4 = reinterpret_cast<const float4*>(col_k + st * BN);
         const float4* v4 = reinterpret_cast<const float4*>(col_v + st * BN);
-        // ---- the block's max
+        const bool all = v0 >= full0 && v0 + BN <= full1;  // the same for the warp
+        uint32_t sees[2] = {0xffffffffu, 0xffffffffu};
+        if (!all) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) sees[c] = mine ? tree_sees(A, node_at, node, start, cnt, n_ring, v0 + 32 * c) : 0u;
+        }
+        if (I8)
+          is_slow |= ((sees[0] & odd[st * NC]) | (sees[1] & odd[st * NC + 1])) != 0;
+        else
+          is_slow |= ((sees[0] & (odd[st * 4] | odd[st * 4 + 2])) | (sees[1] & (odd[st * 4 + 1] | odd[st * 4 + 3]))) != 0;
+        // ---- scores times the key scales, and their max. 64-wide heads keep
+        // them in registers; 128-wide ones, whose outputs fill the registers,
+        // read S twice.
+        constexpr bool KEEP = VP == 64;
+        f32x2 s[KEEP ? 32 : 16];
         float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < NC; ++c) {
-          uint32_t x[2][16];
-          tmem_ld16(s_at + lanes + c * 32, x[0]);
-          tmem_ld16(s_at + lanes + c * 32 + 16, x[1]);
-          const int v = v0 + c * 32;
-          const bool all = v >= full0 && v + 32 <= full1;  // the same for the warp
-          uint32_t sees = 0xffffffffu;
-          if (!all) sees = mine ? tree_sees(A, node_at, node, start, cnt, n_ring, v) : 0u;
-          is_slow |= (sees & odd[st * NC + c]) != 0;
-          tmem_wait_ld();
+        auto scores = [&](const uint32_t (&x)[32], int c, f32x2* to) {  // half c of the sub-block
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float4 k = k4[c * 8 + j];
-            float a, d, e, f;
-            const uint32_t* y = x[j >> 2] + 4 * (j & 3);
-            up(mul2(pk(__uint_as_float(y[0]), __uint_as_float(y[1])), pk(k.x, k.y)), a, d);
-            up(mul2(pk(__uint_as_float(y[2]), __uint_as_float(y[3])), pk(k.z, k.w)), e, f);
-            if (!all) {
-              const uint32_t w = sees >> (4 * j);
-              a = w & 1 ? a : -INFINITY, d = w & 2 ? d : -INFINITY;
-              e = w & 4 ? e : -INFINITY, f = w & 8 ? f : -INFINITY;
+            to[2 * j] = mul2(pk(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1])), pk(k.x, k.y));
+            to[2 * j + 1] = mul2(pk(__uint_as_float(x[4 * j + 2]), __uint_as_float(x[4 * j + 3])), pk(k.z, k.w));
+          }
+          if (!all) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float f0, f1;
+              up(to[j], f0, f1);
+              to[j] = pk((sees[c] >> (2 * j)) & 1 ? f0 : -INFINITY, (sees[c] >> (2 * j + 1)) & 1 ? f1 : -INFINITY);
             }
-            mx = fmaxf(mx, fmaxf(fmaxf(a, d), fmaxf(e, f)));
+          }
+        };
+        auto top_of = [&](const f32x2* a) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float f0, f1;
+            up(a[j], f0, f1);
+            mx = fmaxf(fmaxf(mx, f0), f1);
+          }
+        };
+        if (KEEP) {
+          uint32_t x0[32], x1[32];
+          tmem_ld32(s_now, x0);
+          tmem_ld32(s_now + 32, x1);
+          tmem_landed();
+          scores(x0, 0, s);
+          scores(x1, 1, s + (KEEP ? 16 : 0));
+          top_of(s);
+          top_of(s + (KEEP ? 16 : 0));
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t x[32];
+            tmem_ld32(s_now + 32 * c, x);
+            tmem_landed();
+            scores(x, c, s);
+            top_of(s);
           }
         }
         const float mn = fmaxf(m, mx * qs), mz = mn == -INFINITY ? 0.f : mn;
         const float corr = ex2(m - mz);
         m = mn;
-        // ---- the last block's output, then the new scale
+        // ---- the last sub-block's output, then the new scale
         const int e = expo[2 * st];
         low = expo[2 * st + 1];
         if (it > 0) {
-          if (!mbar_wait(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
+          if (!mbar_wait_asleep(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < VP; c += 16) {
-            uint32_t x[16];
-            tmem_ld16(o_at + lanes + c, x);
-            tmem_wait_ld();
+          for (int c = 0; c < VP; c += 32) {
+            uint32_t x[2][16];
+            tmem_ld16(o_at + lanes + c, x[0]);
+            tmem_ld16(o_at + lanes + c + 16, x[1]);
+            tmem_landed();
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              o[(c + j) / 2] = add2(o[(c + j) / 2], pk(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
-            }
+            for (int j = 0; j < 32; j += 2)
+              o[(c + j) / 2] = add2(o[(c + j) / 2], pk(__uint_as_float(x[j >> 4][j & 15]), __uint_as_float(x[j >> 4][(j & 15) + 1])));
           }
           const float by = corr * (e - e_old > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (e - e_old)) << 23));
           if (__any_sync(0xffffffffu, by != 1.f)) {
@@ -475,45 +501,44 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         }
         e_old = e;
         // ---- weights: sum, and times the value scale as f16 parts into S's place
-        // (16 positions at a time: their 16 columns take 8 of high parts, 8 of remainders)
+        // (16 positions' columns take 8 of high parts, then 8 of remainders)
         f32x2 add = pk(0.f, 0.f);
         const f32x2 qs2 = pk(qs, qs), mz2 = pk(-mz, -mz);
-#pragma unroll 1
-        for (int c = 0; c < 2 * NC; ++c) {
-          uint32_t x[16];
-          tmem_ld16(s_at + lanes + c * 16, x);
-          const int v = v0 + (c >> 1) * 32;
-          const bool all = v >= full0 && v + 32 <= full1;
-          uint32_t seen = 0xffffffffu;
-          if (!all) seen = mine ? tree_sees(A, node_at, node, start, cnt, n_ring, v) >> ((c & 1) * 16) : 0u;
-          tmem_wait_ld();
+        auto weights = [&](const f32x2* a, int c) {  // 16 positions from 16 c
           uint32_t hi[8], lo[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float4 k = k4[c * 4 + j], vv = v4[c * 4 + j];
+            const float4 vv = v4[c * 4 + j];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float a, d;
-              up(fma2(mul2(pk(__uint_as_float(x[4 * j + 2 * h]), __uint_as_float(x[4 * j + 2 * h + 1])),
-                           h ? pk(k.z, k.w) : pk(k.x, k.y)),
-                      qs2, mz2),
-                 a, d);
-              if (!all) {
-                const uint32_t w = seen >> (4 * j + 2 * h);
-                a = w & 1 ? a : -INFINITY, d = w & 2 ? d : -INFINITY;
-              }
-              const f32x2 p = pk(ex2(a), ex2(d));
+            for (int g = 0; g < 2; ++g) {
+              float f0, f1, w0, w1;
+              up(fma2(a[2 * j + g], qs2, mz2), f0, f1);
+              const f32x2 p = pk(ex2(f0), ex2(f1));
               add = add2(add, p);
-              float wa, wd;
-              up(mul2(p, h ? pk(vv.z, vv.w) : pk(vv.x, vv.y)), wa, wd);
-              const float ta = __uint_as_float(__float_as_uint(wa) & 0xffffe000u),
-                          td = __uint_as_float(__float_as_uint(wd) & 0xffffe000u);
-              hi[2 * j + h] = cvt2(ta, td);
-              lo[2 * j + h] = cvt2(wa - ta, wd - td);
+              const f32x2 w = mul2(p, g ? pk(vv.z, vv.w) : pk(vv.x, vv.y));
+              up(w, w0, w1);
+              const float t0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u),
+                          t1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
+              hi[2 * j + g] = cvt2(t0, t1);
+              lo[2 * j + g] = cvt2(w0 - t0, w1 - t1);
             }
           }
-          tmem_st8(s_at + lanes + c * 16, hi);
-          tmem_st8(s_at + lanes + c * 16 + 8, lo);
+          tmem_st8(s_now + c * 16, hi);
+          tmem_st8(s_now + c * 16 + 8, lo);
+        };
+        if (KEEP) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) weights(s + (KEEP ? c * 8 : 0), c);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t x[32];
+            tmem_ld32(s_now + 32 * c, x);
+            tmem_landed();
+            scores(x, c, s);
+            weights(s, 2 * c);
+            weights(s + 8, 2 * c + 1);
+          }
         }
         float a, d;
         up(add, a, d);
@@ -521,18 +546,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         tmem_wait_st();
         tc_fence_before();
       }
-      if (W == 1 || wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-      else asm volatile("bar.sync 2, 128;" ::: "memory");
-      if (issuer && ok) {
-        tc_fence_after();
-        issue_pv(i);
-        // The next S takes the place of this P: only once the product is done.
-        if (i + W < nblk && mbar_wait(&o_full[wg], (uint32_t)it & 1u, abort, werr)) issue_qk(i + W);
-      }
       __syncwarp();
+      if (ok && lane == 0) mbar_arrive(&p_full[wg]);
     }
     if (it > 0) {
-      if (ok && !mbar_wait(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
+      if (ok && !mbar_wait_asleep(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
@@ -543,12 +561,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         float top = 0.f;
         bool bad = false;
 #pragma unroll
-        for (int c = 0; c < VP; c += 16) {
-          uint32_t x[16];
-          tmem_ld16(o_at + lanes + c, x);
+        for (int c = 0; c < VP; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(o_at + lanes + c, x);
           tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
+          for (int j = 0; j < 32; j += 2) {
             const f32x2 t = add2(o[(c + j) / 2], pk(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
             float t0, t1;
             up(t, t0, t1);
@@ -565,11 +583,6 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         is_slow = false;
       }
     }
-    if (issuer) {  // every issued MMA completes before TMEM is freed
-      umma_commit(&drain[wg]);
-      mbar_drain(&drain[wg], 0);
-    }
-    __syncwarp();
     if (mine && is_slow) atomicOr(&slow[r >> 5], 1u << (r & 31));
     // ---- merge the warpgroups (every block is consumed: the stages' memory is
     // free) and write
@@ -610,233 +623,371 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         float* dst = A.out + (node_at * A.heads + head) * A.vh;
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int d = 0; d < VP; d += 2)  // vh and the start of out are multiples of two floats
-          if (d < A.vh) *reinterpret_cast<f32x2*>(dst + d) = mul2(o[d / 2], pk(inv, inv));
+        for (int d = 0; d < VP; d += 4)  // vh and the start of out are multiples of four floats
+          if (d < A.vh)
+            *reinterpret_cast<ulonglong2*>(dst + d) =
+                make_ulonglong2(mul2(o[d / 2], pk(inv, inv)), mul2(o[d / 2 + 1], pk(inv, inv)));
       }
     }
   } else {
-    // ------------------------------------------------------------ producers
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_PROD));
-    const int p = tid - W * 128, pw = p >> 5;
-    bool ok = true;
-    int e = 14, low = 255;
-    for (int i = 0; i < nblk; ++i) {
-      const int st = i % NST, v0 = (blk0 + i) * BN;
-      unsigned char* kt = stages + (size_t)st * C::STAGE;
-      unsigned char* vt = kt + C::PARTS * C::K_TILE;
-      const bool wait_empty = ok;
-      if (I8) {
-        // Keys: a position a thread. Values: eight positions (octet) by VP / 8
-        // dims a thread; a warp reads whole sectors and writes one 16-byte
-        // chunk of eight positions per dim, lanes in different chunks.
-        constexpr int DV = VP / 8;  // dims of a thread
-        const int v = v0 + p, pr = (pw & 1) * 8 + (lane & 7), d0 = ((pw >> 1) * 4 + (lane >> 3)) * DV;
-        uint4 k[QS];
-        uint32_t x[8][DV / 4];
-        float ksc = 0.f, vsc = 0.f;
-        {
-          const bool in = v < P.total;
-          const bool d = P.in_draft(v);
+    const int role = warp & 3, set = wg - W;  // 0 keys, 1 and 2 values of the steps of warpgroup `set`, 3 MMA
+    if (role == 3 && set > 0) {
+      // nothing to do
+    } else if (role == 3) {
+      // ---------------------------------------------------------- MMA issue
+      const uint64_t dq_hi = sw128_desc(qhi), dq_lo = sw128_desc(qlo), d_stage = sw128_desc(stages);
+      auto issue_qk = [&](int i) {  // S of step i
+        const int st = i % NST, w = i % W, jj = i / W;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dk = d_stage + (uint64_t)(st * (C::STAGE >> 4));
+          const uint32_t d = tmem + w * C::WG_COLS + (jj & 1) * BN;
+          uint32_t acc = 0;
+          auto steps = [&](uint64_t dq, uint64_t dkk) {
+#pragma unroll
+            for (int k = 0; k < QS; ++k) {
+              mma_ss<BN>(d, dq + (uint64_t)((k >> 2) * (128 * 128 >> 4) + (k & 3) * 2),
+                         dkk + (uint64_t)((k >> 2) * (BN * 128 >> 4) + (k & 3) * 2), acc);
+              acc = 1;
+            }
+          };
+          steps(dq_lo, dk);
+          if (!I8) steps(dq_hi, dk + (uint64_t)(C::K_TILE >> 4));
+          steps(dq_hi, dk);
+          umma_commit(&s_full[2 * w + (jj & 1)]);
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](int i) {  // O of step i
+        const int st = i % NST, w = i % W, jj = i / W;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dv = d_stage + (uint64_t)((st * C::STAGE + C::PARTS * C::K_TILE) >> 4);
+          const uint32_t at = tmem + w * C::WG_COLS, p = at + (jj & 1) * BN;
+          uint32_t acc = 0;
+          auto steps = [&](uint32_t a, uint64_t dvv) {
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k) {
+              mma_ts<VP>(at + 2 * BN, a + k * 16, dvv + (uint64_t)(k * 2), acc);
+              acc = 1;
+            }
+          };
+          steps(p + 8, dv);
+          if (!I8) steps(p, dv + (uint64_t)(C::V_TILE >> 4));
+          steps(p, dv);
+          umma_commit(&o_full[w]);
+          umma_commit(&empty[st]);
+        }
+        __syncwarp();
+      };
+      // The scores of the first two steps of a warpgroup, then after each second
+      // product scores again: they take the place of the weights of step q - 2 W,
+      // whose product must be done. With two warpgroups they follow one product
+      // later, so that the wait for it is over when it begins.
+      auto scores = [&](int q) {
+        bool ready = mbar_wait_asleep(&full[q % NST], (uint32_t)(q / NST) & 1u, abort, werr);
+        if (ready && q >= 2 * W) ready = mbar_wait_asleep(&o_full[q % W], (uint32_t)(q / W) & 1u, abort, werr);
+        ready = __all_sync(0xffffffffu, ready);
+        if (ready) issue_qk(q);
+        return ready;
+      };
+      bool ok = nblk == 0 || mbar_wait_asleep(q_full, 0, abort, werr);
+      ok = __all_sync(0xffffffffu, ok);
+      constexpr int AHEAD = 2 * W - (W - 1);  // steps from a second product to the scores issued after it
+      for (int q = 0; q < AHEAD && q < nblk && ok; ++q) ok = scores(q);
+      for (int i = 0; i < nblk && ok; ++i) {
+        ok = mbar_wait_asleep(&p_full[i % W], (uint32_t)(i / W) & 1u, abort, werr);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) issue_pv(i);
+        if (ok && i + AHEAD < nblk) ok = scores(i + AHEAD);
+      }
+      // Every issued MMA completes before TMEM is freed.
+      if (elect_one()) umma_commit(drain);
+      __syncwarp();
+      mbar_drain(drain, 0);
+    } else if (role == 0) {
+      // ---------------------------------------------------------- keys and scales
+      bool ok = true;
+      int e = 14, low = 255;
+      // int8: positions lane and lane + 32 of a step and their scales; the next
+      // step's are on their way while one is widened (of wide keys, whose second
+      // set of warps is at work meanwhile, none).
+      constexpr bool AHEAD = I8 && W == 1;
+      uint4 kn[2][QS];
+      float ksn[2], vsn[2];
+      auto load = [&](int i) {
+        const int v0 = (blk0 + i) * BN;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int v = v0 + h * 32 + lane;
+          const bool in = v < P.total, d = P.in_draft(v);
           const size_t row = in ? P.row(v) : 0;
-          if (in) ksc = (d ? A.tks : A.ks)[row], vsc = (d ? A.tvs : A.vs)[row];
-          const char* src = (d ? A.tk : A.k) + row * A.qk;
+          ksn[h] = in ? __ldg((d ? A.tks : A.ks) + row) : 0.f;
+          vsn[h] = in ? __ldg((d ? A.tvs : A.vs) + row) : 0.f;
+          const uint4* src = reinterpret_cast<const uint4*>((d ? A.tk : A.k) + row * A.qk);
+          if (AHEAD || h == 0) {
 #pragma unroll
-          for (int c = 0; c < QS; ++c)
-            k[c] = in && c * 16 < A.qk ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int vj = v0 + pr * 8 + j;
-          const bool in = vj < P.total && d0 < A.vh;
-          const char* src = (P.in_draft(vj) ? A.tv : A.v) + (in ? P.row(vj) : 0) * A.vh + d0;
-          if (DV == 8) {
-            const uint2 t = in ? __ldg(reinterpret_cast<const uint2*>(src)) : make_uint2(0, 0);
-            x[j][0] = t.x, x[j][1] = t.y;
-          } else {
-            const uint4 t = in ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
-            x[j][0] = t.x, x[j][1] = t.y, x[j][DV / 4 - 2] = t.z, x[j][DV / 4 - 1] = t.w;
+            for (int c = 0; c < QS; ++c) kn[h][c] = in && c * 16 < A.qk ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
           }
         }
-        if (wait_empty && !mbar_wait(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
-        // scales
-        const bool sane = fabsf(ksc) <= 3.4028234e38f && fabsf(vsc) <= 3.4028234e38f;
-        const uint32_t oddw = __ballot_sync(0xffffffffu, !sane);
-        if (!sane) vsc = 0.f;
-        const uint32_t vb = __float_as_uint(fabsf(vsc));
-        const uint32_t hi = __reduce_max_sync(0xffffffffu, vb),
-                       lo = __reduce_min_sync(0xffffffffu, vb ? vb : 0x7f800000u);
-        uint32_t* wm = reinterpret_cast<uint32_t*>(wmax) + (i & 1) * 8;
-        if (lane == 0) wm[pw] = hi, wm[4 + pw] = lo;
-        if (lane == 0) odd[st * NC + pw] = oddw;
-        asm volatile("bar.sync 4, 128;" ::: "memory");
-        e = min(max(e, (int)(max(max(wm[0], wm[1]), max(wm[2], wm[3])) >> 23)), 253);
-        low = min(low, (int)(min(min(wm[4], wm[5]), min(wm[6], wm[7])) >> 23));
-        col_k[st * BN + p] = ksc;
-        col_v[st * BN + p] = vsc * __uint_as_float((uint32_t)(267 - e) << 23);
-        if (p == 0) expo[2 * st] = e, expo[2 * st + 1] = low;
-        // keys
-#pragma unroll
-        for (int c = 0; c < QS; ++c) {
-          uint32_t w[8];
-          widen(k[c].x ^ 0x80808080u, &w[0], &w[1]);
-          widen(k[c].y ^ 0x80808080u, &w[2], &w[3]);
-          widen(k[c].z ^ 0x80808080u, &w[4], &w[5]);
-          widen(k[c].w ^ 0x80808080u, &w[6], &w[7]);
-          unsigned char* row = kt + (c >> 2) * (BN * 128) + p * 128;
-          *reinterpret_cast<uint4*>(row + ((((c & 3) * 2) ^ (p & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + 1) ^ (p & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
-        }
-        // values, transposed: dims 2g, 2g + 1 of two positions in one permute
-        if (d0 < A.vh) {
-#pragma unroll
-          for (int q = 0; q < DV / 4; ++q) {
-            uint32_t w[4][4];  // [dim][position pair]
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t a = x[2 * j][q] ^ 0x80808080u, c = x[2 * j + 1][q] ^ 0x80808080u;
-              widen(__byte_perm(a, c, 0x5140), &w[0][j], &w[1][j]);
-              widen(__byte_perm(a, c, 0x7362), &w[2][j], &w[3][j]);
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const int d = d0 + 4 * q + t;
-              *reinterpret_cast<uint4*>(vt + (pr >> 3) * (VP * 128) + d * 128 + (((pr & 7) ^ (d & 7)) << 4)) =
-                  make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
-            }
-          }
-        }
-      } else {
-        // f32, BN = 64. Keys: two threads a position. Values: eight positions
-        // by four dims a thread.
-        constexpr int HC = QS;  // 8-dim chunks of half a key row
-        const int kp = p >> 1, half = p & 1, v = v0 + kp;
-        const int pr = lane & 7, d0 = (pw * 4 + (lane >> 3)) * 4;
-        float4 x[8];
-        bool sane = true;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int vj = v0 + pr * 8 + j;
-          const bool in = vj < P.total && d0 < A.vh;
-          const float* src =
-              reinterpret_cast<const float*>(P.in_draft(vj) ? A.tv : A.v) + (in ? P.row(vj) : 0) * A.vh + d0;
-          x[j] = in ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0, 0, 0, 0);
-        }
-        if (wait_empty && !mbar_wait(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
-        float ksc;
-        {
-          const bool in = v < P.total;
-          const float* src = reinterpret_cast<const float*>(P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk;
-          float4 k[HC][2];
-          float mx = 0.f;
-#pragma unroll
-          for (int c = 0; c < HC; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int d = (half * HC + c) * 8 + 4 * h;
-              k[c][h] = in && d < A.qk ? __ldg(reinterpret_cast<const float4*>(src + d)) : make_float4(0, 0, 0, 0);
-              mx = fmaxf(mx, fmaxf(fmaxf(fabsf(k[c][h].x), fabsf(k[c][h].y)), fmaxf(fabsf(k[c][h].z), fabsf(k[c][h].w))));
-              sane &= fabsf(k[c][h].x) <= 3.4028234e38f && fabsf(k[c][h].y) <= 3.4028234e38f &&
-                      fabsf(k[c][h].z) <= 3.4028234e38f && fabsf(k[c][h].w) <= 3.4028234e38f;
-            }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          const int ef = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
-          const float by = __uint_as_float((uint32_t)(267 - ef) << 23);  // max into [2^13, 2^14)
-          ksc = __uint_as_float((uint32_t)(ef - 13) << 23);
-#pragma unroll
-          for (int c = 0; c < HC; ++c) {
-            uint32_t hh[4], ll[4];
-            halves(k[c][0].x * by, k[c][0].y * by, &hh[0], &ll[0]);
-            halves(k[c][0].z * by, k[c][0].w * by, &hh[1], &ll[1]);
-            halves(k[c][1].x * by, k[c][1].y * by, &hh[2], &ll[2]);
-            halves(k[c][1].z * by, k[c][1].w * by, &hh[3], &ll[3]);
-            const int ch = half * HC + c;
-            unsigned char* at = kt + (ch >> 3) * (BN * 128) + kp * 128 + (((ch & 7) ^ (kp & 7)) << 4);
-            *reinterpret_cast<uint4*>(at) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
-            *reinterpret_cast<uint4*>(at + C::K_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
-          }
-        }
-        uint32_t oddk = __ballot_sync(0xffffffffu, !sane);  // two lanes a position: positions 16 pw ..
-        // largest value of each position: over the warp's dims, then the warps'
-        float* wm = wmax + (i & 1) * 256;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float a = fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
-          // NaN and infinity both read as infinity
-          const float s = fabsf(x[j].x) + fabsf(x[j].y) + fabsf(x[j].z) + fabsf(x[j].w);
-          if (!(a <= 3.4028234e38f) || s != s) a = INFINITY;
-          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 8));
-          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 16));
-          if (lane < 8) wm[pw * 64 + pr * 8 + j] = a;
-        }
-        uint32_t* om = odd + st * NC;
-        if (p < NC) om[p] = 0;
-        asm volatile("bar.sync 4, 128;" ::: "memory");
-        float mxs[8];
-        int top = 0, least = 255;
-        uint32_t bad = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int at = pr * 8 + j;
-          const float a = fmaxf(fmaxf(wm[at], wm[64 + at]), fmaxf(wm[128 + at], wm[192 + at]));
-          mxs[j] = a;
-          if (a == INFINITY) {
-            bad |= 1u << j;
-          } else if (a > 0.f) {
-            const int f = min(max((int)(__float_as_uint(a) >> 23), 14), 253) - 13;
-            top = max(top, f), least = min(least, f);
-          }
-        }
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) {
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-          least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
-        }
-        e = max(e, top), low = min(low, least);
-        // odd columns: bits 8 (pr % 4) + j of word pr / 4 for values, spread pairs for keys
-        if (pw == 0 && lane < 8 && bad) atomicOr(&om[pr >> 2], bad << ((pr & 3) * 8));
-        if (lane == 0 && oddk) {
-          uint32_t w = 0;
-          for (int j = 0; j < 16; ++j)
-            if ((oddk >> (2 * j)) & 3u) w |= 1u << j;
-          atomicOr(&om[pw >> 1], w << ((pw & 1) * 16));
-        }
-        if (half == 0) col_k[st * BN + kp] = v < P.total ? ksc : 0.f;
-        if (p == 0) expo[2 * st] = e, expo[2 * st + 1] = low;
-        uint32_t hh[4][4], ll[4][4];  // [dim][position pair]
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float by[2];
+      };
+      if (I8 && set < nblk) load(set);
+      for (int i = set; i < nblk; i += W) {
+        const int st = i % NST, v0 = (blk0 + i) * BN;
+        unsigned char* kt = stages + (size_t)st * C::STAGE;
+        float ksc[2], vsc[2];
+        bool sane[2];
+        if (I8) {
+          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          __syncwarp();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float a = mxs[2 * j + h];
-            const int ef = min(max((int)(__float_as_uint(a) >> 23), 14), 253);
-            const bool use = a > 0.f && a != INFINITY;
-            by[h] = use ? __uint_as_float((uint32_t)(267 - ef) << 23) : 0.f;
-            // value scale 2^(ef - 140) times 2^(140 - e): exponent ef - 13 below e
-            const int f = 127 + 13 + ef - 13 - e;
-            if (pw == 0 && lane < 8)
-              col_v[st * BN + pr * 8 + 2 * j + h] = use && f > 0 ? __uint_as_float((uint32_t)f << 23) : 0.f;
-          }
-          const float4 a = x[2 * j], c = x[2 * j + 1];
-          const bool ua = by[0] != 0.f, uc = by[1] != 0.f;
-          halves(ua ? a.x * by[0] : 0.f, uc ? c.x * by[1] : 0.f, &hh[0][j], &ll[0][j]);
-          halves(ua ? a.y * by[0] : 0.f, uc ? c.y * by[1] : 0.f, &hh[1][j], &ll[1][j]);
-          halves(ua ? a.z * by[0] : 0.f, uc ? c.z * by[1] : 0.f, &hh[2][j], &ll[2][j]);
-          halves(ua ? a.w * by[0] : 0.f, uc ? c.w * by[1] : 0.f, &hh[3][j], &ll[3][j]);
-        }
-        if (d0 < A.vh) {
+            const int kp = h * 32 + lane;
+            ksc[h] = ksn[h], vsc[h] = vsn[h];
+            uint4 kk[QS];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int d = d0 + t;
-            unsigned char* at = vt + d * 128 + ((pr ^ (d & 7)) << 4);
-            *reinterpret_cast<uint4*>(at) = make_uint4(hh[t][0], hh[t][1], hh[t][2], hh[t][3]);
-            *reinterpret_cast<uint4*>(at + C::V_TILE) = make_uint4(ll[t][0], ll[t][1], ll[t][2], ll[t][3]);
+            for (int c = 0; c < QS; ++c) kk[c] = kn[AHEAD ? h : 0][c];
+            if (!AHEAD && h == 0) {
+              const int v = v0 + 32 + lane;
+              const bool in = v < P.total;
+              const uint4* src =
+                  reinterpret_cast<const uint4*>((P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk);
+#pragma unroll
+              for (int c = 0; c < QS; ++c) kn[0][c] = in && c * 16 < A.qk ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+            }
+            if (AHEAD && h == 1 && i + W < nblk) load(i + W);
+#pragma unroll
+            for (int c = 0; c < QS; ++c) {
+              uint32_t w[8];
+              widen(kk[c].x ^ 0x80808080u, &w[0], &w[1]);
+              widen(kk[c].y ^ 0x80808080u, &w[2], &w[3]);
+              widen(kk[c].z ^ 0x80808080u, &w[4], &w[5]);
+              widen(kk[c].w ^ 0x80808080u, &w[6], &w[7]);
+              unsigned char* row = kt + (c >> 2) * (BN * 128) + kp * 128;
+              *reinterpret_cast<uint4*>(row + ((((c & 3) * 2) ^ (kp & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + 1) ^ (kp & 7)) << 4)) =
+                  make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            sane[h] = fabsf(ksc[h]) <= 3.4028234e38f && fabsf(vsc[h]) <= 3.4028234e38f;
+          }
+          if (!AHEAD && i + W < nblk) load(i + W);
+          // Value scales, held so that the largest so far is in [2^13, 2^14).
+          uint32_t top = 0, least = 0x7f800000u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!sane[h]) vsc[h] = 0.f;
+            const uint32_t a = __float_as_uint(fabsf(vsc[h]));
+            top = max(top, a), least = min(least, a ? a : 0x7f800000u);
+          }
+          e = min(max(e, (int)(__reduce_max_sync(0xffffffffu, top) >> 23)), 253);
+          low = min(low, (int)(__reduce_min_sync(0xffffffffu, least) >> 23));
+          const float f = __uint_as_float((uint32_t)(267 - e) << 23);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            col_k[st * BN + h * 32 + lane] = ksc[h];
+            col_v[st * BN + h * 32 + lane] = vsc[h] * f;
+            const uint32_t w = __ballot_sync(0xffffffffu, !sane[h]);
+            if (lane == 0) odd[st * NC + h] = w;
+          }
+          if (lane == 0) expo[2 * st] = e, expo[2 * st + 1] = low;
+        } else {
+          // f32: each key scaled by the power of two that brings its largest
+          // element into [2^13, 2^14); the values' scales are the value warps' matter.
+          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          __syncwarp();
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const int kp = h * 32 + lane, v = v0 + kp;
+            const bool in = v < P.total;
+            const float4* src = reinterpret_cast<const float4*>(
+                reinterpret_cast<const float*>(P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk);
+            // Twice over the row (the second time from cache): its largest element, then its parts.
+            float mx = 0.f;
+            bool fine = true;
+#pragma unroll 4
+            for (int c = 0; c < QS * 4; ++c) {
+              const float4 f = in && c * 4 < A.qk ? __ldg(src + c) : make_float4(0, 0, 0, 0);
+              const float a = fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w)));
+              const float t = fabsf(f.x) + fabsf(f.y) + fabsf(f.z) + fabsf(f.w);  // NaN where one is
+              fine &= a <= 3.4028234e38f && t == t;
+              mx = fmaxf(mx, a);
+            }
+            const int ef = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
+            const float by = __uint_as_float((uint32_t)(267 - ef) << 23);
+#pragma unroll 2
+            for (int c = 0; c < QS * 2; ++c) {
+              const float4 f = in && c * 8 < A.qk ? __ldg(src + 2 * c) : make_float4(0, 0, 0, 0);
+              const float4 g = in && c * 8 < A.qk ? __ldg(src + 2 * c + 1) : make_float4(0, 0, 0, 0);
+              uint32_t hh[4], ll[4];
+              halves(f.x * by, f.y * by, &hh[0], &ll[0]);
+              halves(f.z * by, f.w * by, &hh[1], &ll[1]);
+              halves(g.x * by, g.y * by, &hh[2], &ll[2]);
+              halves(g.z * by, g.w * by, &hh[3], &ll[3]);
+              unsigned char* at = kt + kp * 128 + ((c ^ (kp & 7)) << 4);
+              *reinterpret_cast<uint4*>(at) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
+              *reinterpret_cast<uint4*>(at + C::K_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
+            }
+            col_k[st * BN + kp] = in ? __uint_as_float((uint32_t)(ef - 13) << 23) : 0.f;
+            const uint32_t w = __ballot_sync(0xffffffffu, !fine);
+            if (lane == 0) odd[st * 2 * NC + h] = w;
           }
         }
-        asm volatile("bar.sync 4, 128;" ::: "memory");  // the odd words are whole
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&full[st]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&full[st]);
+    } else {
+      // ---------------------------------------------------------- values
+      const int vw = role - 1;
+      bool ok = true;
+      int e = 14, low = 255;
+      // int8: eight positions (an octet) by VP / 8 dims a thread: a warp reads
+      // whole sectors and writes one 16-byte chunk of eight positions per dim, its
+      // lanes in different chunks. The next step's values are on their way while
+      // one is widened.
+      constexpr int DV = VP / 8;
+      constexpr bool AHEAD = I8 && W == 1;
+      const int d0 = (vw * 4 + (lane >> 3)) * DV;
+      uint32_t xn[8][DV / 4];
+      auto get = [&](const char* src, bool in, uint32_t (&x)[DV / 4]) {
+        if (DV == 8) {
+          const uint2 t = in ? __ldg(reinterpret_cast<const uint2*>(src)) : make_uint2(0, 0);
+          x[0] = t.x, x[1] = t.y;
+        } else {
+          const uint4 t = in ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+          x[0] = t.x, x[1] = t.y, x[DV / 4 - 2] = t.z, x[DV / 4 - 1] = t.w;
+        }
+      };
+      auto load = [&](int i) {
+        const int v = (blk0 + i) * BN + (lane & 7) * 8;
+        if (P.plain((blk0 + i) * BN, BN)) {  // the same for the warp
+          const char* src = A.v + P.row(v) * A.vh + d0;
+          const size_t step = (size_t)A.kvh * A.vh;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) get(src + j * step, d0 < A.vh, xn[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool in = v + j < P.total && d0 < A.vh;
+            get((P.in_draft(v + j) ? A.tv : A.v) + (in ? P.row(v + j) : 0) * A.vh + (in ? d0 : 0), in, xn[j]);
+          }
+        }
+      };
+      if (I8 && set < nblk) load(set);
+      for (int i = set; i < nblk; i += W) {
+        const int st = i % NST, v0 = (blk0 + i) * BN;
+        unsigned char* vt = stages + (size_t)st * C::STAGE + C::PARTS * C::K_TILE;
+        if (I8) {
+          const int pr = lane & 7;
+          uint32_t x[8][DV / 4];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int q = 0; q < DV / 4; ++q) x[j][q] = xn[j][q];
+          if (AHEAD && i + W < nblk) load(i + W);
+          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          __syncwarp();
+          if (d0 < A.vh) {
+#pragma unroll
+            for (int q = 0; q < DV / 4; ++q) {
+              uint32_t w[4][4];  // [dim][position pair]
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t a = x[2 * j][q] ^ 0x80808080u, c = x[2 * j + 1][q] ^ 0x80808080u;
+                widen(__byte_perm(a, c, 0x5140), &w[0][j], &w[1][j]);
+                widen(__byte_perm(a, c, 0x7362), &w[2][j], &w[3][j]);
+              }
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                const int d = d0 + 4 * q + t;
+                *reinterpret_cast<uint4*>(vt + d * 128 + ((pr ^ (d & 7)) << 4)) =
+                    make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
+              }
+            }
+          }
+          if (!AHEAD && i + W < nblk) load(i + W);
+        } else {
+          // f32: a warp holds 32 positions (four octets) whole, four dims a lane
+          // in each of two rounds, so a position's largest value is the warp's
+          // own matter. A value is scaled like a key; 2^(140 - e) is a step's
+          // share of the scale, by the largest exponent of both warps so far.
+          const int oc = lane & 3, pr = vw * 4 + oc;
+          auto row_of = [&](int j) {  // position j of the octet, null past the end
+            const int vj = v0 + pr * 8 + j;
+            return vj < P.total ? reinterpret_cast<const float*>(P.in_draft(vj) ? A.tv : A.v) + P.row(vj) * A.vh : nullptr;
+          };
+          auto at = [&](const float* row, int d) {
+            return row && d < A.vh ? __ldg(reinterpret_cast<const float4*>(row + d)) : make_float4(0, 0, 0, 0);
+          };
+          // Twice over the values (the second time from cache): exponent field of
+          // each position's largest (0 none, 255 not finite), then the parts.
+          int top = 0, least = 255;
+          uint32_t ef[2] = {0, 0}, bad = 0;  // a byte a position
+#pragma unroll 2
+          for (int j = 0; j < 8; ++j) {
+            const float* row = row_of(j);
+            const float4 f = at(row, (lane >> 2) * 4), g = at(row, 32 + (lane >> 2) * 4);
+            float a = fmaxf(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))),
+                            fmaxf(fmaxf(fabsf(g.x), fabsf(g.y)), fmaxf(fabsf(g.z), fabsf(g.w))));
+            const float t = fabsf(f.x) + fabsf(f.y) + fabsf(f.z) + fabsf(f.w) + fabsf(g.x) + fabsf(g.y) + fabsf(g.z) +
+                            fabsf(g.w);  // NaN where one is
+            if (t != t) a = INFINITY;
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+            const int x = a == 0.f ? 0 : a <= 3.4028234e38f ? min(max((int)(__float_as_uint(a) >> 23), 14), 253) : 255;
+            if (x == 255) bad |= 1u << (8 * oc + j);
+            else if (x > 0) top = max(top, x - 13), least = min(least, x - 13);
+            ef[j >> 2] |= (uint32_t)x << (8 * (j & 3));
+          }
+          top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
+          bad = __reduce_or_sync(0xffffffffu, bad);
+          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          __syncwarp();
+          if (lane == 0) vmax[(i & 1) * 4 + vw] = top, vmax[(i & 1) * 4 + 2 + vw] = least;
+          asm volatile("bar.sync 4, 64;" ::: "memory");
+          e = max(e, max(vmax[(i & 1) * 4], vmax[(i & 1) * 4 + 1]));
+          low = min(low, min(vmax[(i & 1) * 4 + 2], vmax[(i & 1) * 4 + 3]));
+          if (lane == 0) odd[st * 2 * NC + NC + vw] = bad;
+          if (vw == 0 && lane == 0) expo[2 * st] = e, expo[2 * st + 1] = low;
+          if (lane < 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int x = (int)((ef[j >> 2] >> (8 * (j & 3))) & 255u), f = 127 + x - e;  // 2^(x - 140) 2^(140 - e)
+              col_v[st * BN + pr * 8 + j] = x > 0 && x < 255 && f > 0 ? __uint_as_float((uint32_t)f << 23) : 0.f;
+            }
+          }
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const int d0 = h * 32 + (lane >> 2) * 4;
+            float4 x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int y = (int)((ef[j >> 2] >> (8 * (j & 3))) & 255u);
+              const bool use = y > 0 && y < 255;  // nothing of one that is not finite
+              const float by = use ? __uint_as_float((uint32_t)(267 - y) << 23) : 0.f;
+              x[j] = at(use ? row_of(j) : nullptr, d0);
+              x[j].x *= by, x[j].y *= by, x[j].z *= by, x[j].w *= by;
+            }
+            if (d0 >= A.vh) continue;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              uint32_t hh[4], ll[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 a = x[2 * j], c = x[2 * j + 1];
+                halves(t == 0 ? a.x : t == 1 ? a.y : t == 2 ? a.z : a.w, t == 0 ? c.x : t == 1 ? c.y : t == 2 ? c.z : c.w,
+                       &hh[j], &ll[j]);
+              }
+              const int d = d0 + t;
+              unsigned char* to = vt + d * 128 + ((pr ^ (d & 7)) << 4);
+              *reinterpret_cast<uint4*>(to) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
+              *reinterpret_cast<uint4*>(to + C::V_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
+            }
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&full[st]);
+      }
     }
   }
   tc_fence_before();
@@ -896,11 +1047,11 @@ cudaError_t launch_umma_form(const TreeArgs& A, int B, cudaStream_t st) {
   return cudaSuccess;
 }
 
-typedef TreeUmma<true, 3, 64, 1, 128, 2> UmmaI8x48;
-typedef TreeUmma<true, 4, 64, 1, 128, 2> UmmaI8x64;
-typedef TreeUmma<true, 8, 128, 2, 128, 2> UmmaI8x128;
-typedef TreeUmma<false, 3, 64, 1, 64, 2> UmmaF32x48;
-typedef TreeUmma<false, 4, 64, 1, 64, 2> UmmaF32x64;
+typedef TreeUmma<true, 3, 64, 1, 4> UmmaI8x48;
+typedef TreeUmma<true, 4, 64, 1, 4> UmmaI8x64;
+typedef TreeUmma<true, 8, 128, 2, 4> UmmaI8x128;
+typedef TreeUmma<false, 3, 64, 1, 2> UmmaF32x48;
+typedef TreeUmma<false, 4, 64, 1, 2> UmmaF32x64;
 
 }  // namespace
 
@@ -911,10 +1062,10 @@ bool tree_umma_takes(int int8, int rows, int qk, int vh, int piece) {
 
 // Splits that need the fewest rounds of blocks: a block of positions costs
 // about 1, a CTA's start and end about 4.
-int tree_umma_nsplit(int int8, int B, int rows, int kvh, int qk, int vh, int span) {
+int tree_umma_nsplit(int B, int rows, int kvh, int qk, int vh, int span) {
   const bool wide = qk > 64 || vh > 64;
   const long work = (long)B * kvh * ((rows + 127) / 128), room = 148 * (wide ? 1 : 2);
-  const int bn = int8 ? 128 : 64, blocks = (span + bn - 1) / bn;
+  const int blocks = (span + 63) / 64;
   int best = 1;
   double cost = 1e300;
   for (int ns = 1; ns <= 128 && ns <= blocks; ++ns) {
