@@ -354,8 +354,8 @@ int nd_attend_tree(const float *q, int ldq, const void *k, const void *v, const 
  * row r: a token that occurs in hist[hist_off[r] .. hist_off[r + 1]) is divided
  * by repetition[r] when positive, else multiplied; one that occurs c > 0 times
  * from hist[gen_from[r]] on (NULL: in all of it) loses c * frequency[r] +
- * presence[r]; the biases of bias_ids[bias_off[r] .. bias_off[r + 1]) are
- * added, in list order where an id repeats; a token whose bit (id % 32 of
+ * presence[r] (c below 2^22); the biases of bias_ids[bias_off[r] ..
+ * bias_off[r + 1]) are added, an id's summed in list order; a token whose bit (id % 32 of
  * mask[r * mask_ld + id / 32]) is clear becomes `masked` (the grammar mask of
  * needle_tokenizer_tool_mask uses -1e9; -INFINITY removes it from any
  * softmax). All arrays are device memory. hist, bias_ids and mask may each be

@@ -1192,10 +1192,9 @@ int nd_attend_tree(const float* q, int ldq, const void* k, const void* v, const 
     return nd_refuse("nd_attend_tree: cache pointers must be 4-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
   const nb::TreePlan plan = nb::tree_plan(k, v, tk, tv, out, int8, B, T, heads, kv_heads, qk, vh, slots);
-  const int ns = plan.nsplit;
   float* part = nullptr;
-  if (ns > 1) {
-    cudaError_t e = scratch_alloc((void**)&part, nb::tree_part_floats(B, T, heads, vh, ns) * 4, st);
+  if (plan.part) {
+    cudaError_t e = scratch_alloc((void**)&part, nb::tree_part_floats(B, T, heads, vh, plan.nsplit) * 4, st);
     if (e != cudaSuccess) return nd_status(e);
   }
   cudaError_t e = nb::launch_attend_tree(q, ldq, k, v, ks, vs, int8, slots, lo, hi, tk, tv, tks, tvs, mask, B, T,

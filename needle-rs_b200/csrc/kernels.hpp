@@ -243,6 +243,7 @@ struct TreePlan {
   bool umma;   // tcgen05 form (tree_umma.cu)
   int piece;   // bytes of a copy the cache's alignment allows
   int nsplit;  // position splits
+  bool part;   // whether they meet in scratch (`part`)
 };
 TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv, const float* out, int int8, int B,
                    int T, int heads, int kvh, int qk, int vh, int slots);

@@ -10,7 +10,9 @@
 
 namespace nb {
 
-inline cudaError_t allow_smem(const void* kern, size_t smem) {
+// most_shared: give shared memory the SM's whole carve-out, for kernels whose
+// blocks share an SM only then.
+inline cudaError_t allow_smem(const void* kern, size_t smem, bool most_shared = false) {
   if (smem == 0) return cudaSuccess;
   static std::mutex mu;
   static std::map<std::pair<const void*, int>, size_t> done;
@@ -25,6 +27,8 @@ inline cudaError_t allow_smem(const void* kern, size_t smem) {
   // included) once; later launches need no call.
   cudaFuncAttributes fa;
   e = cudaFuncGetAttributes(&fa, kern);
+  if (e == cudaSuccess && most_shared)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return e;
   if (smem + fa.sharedSizeBytes <= 48 * 1024) {
     done[key] = smem;

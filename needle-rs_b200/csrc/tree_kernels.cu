@@ -14,6 +14,8 @@
 // f16 values exactly, the query and the softmax weights go in as an f16 high
 // part and remainder (22 bits); f32 rings as three TF32 products of high parts
 // and remainders. Sums, max and the outputs are f32.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "kernels.hpp"
@@ -31,6 +33,7 @@ __device__ __forceinline__ int tree_dim(int n, int col) {
   return I8 ? (n >> 1) * 16 + 2 * col + (n & 1) : n * 8 + col;
 }
 
+constexpr int TREE_CLUSTER = 8;  // blocks of a portable cluster
 constexpr int TREE_WARPS = 4;
 constexpr int TREE_THREADS = TREE_WARPS * 32;
 
@@ -145,7 +148,7 @@ __device__ __forceinline__ void tree_copy(char* buf, const char* k, const char* 
 // the ring's (offsets 0 .. n_ring - 1 from the tile's lowest position) and
 // then the draft's nodes.
 template <bool I8, int QKP, int VHP, int MT>
-__global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const TreeArgs A, int piece) {
+__global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const TreeArgs A, int piece, int cluster) {
   using TT = TreeTile<I8, QKP, VHP>;
   constexpr int PB = TT::PB, NT = PB / 8;        // 8-position score tiles of a block
   constexpr int KC = QKP / 16, VN = VHP / 8;     // 16-dim chunks of a key, 8-dim tiles of an output
@@ -616,11 +619,14 @@ again:
     if (t == 0) row[VHP] = mx[i], row[VHP + 1] = sum[i];
   }
   __syncthreads();
-  const int width = A.nsplit > 1 ? A.vh + 2 : A.vh;
+  // Splits of a cluster: each block leaves its rows (outputs, max, sum) in warp
+  // 0's place, then the blocks share the rows out and read one another's.
+  const bool split = A.nsplit > 1;
+  const int width = split ? A.vh + 2 : A.vh;
+  const size_t ws = (size_t)MT * 16 * PW;
   for (int i = tid; i < rows * width; i += TREE_THREADS) {
     const int r = i / width, d = i - r * width;
     const float* p = P + (size_t)r * PW;
-    const size_t ws = (size_t)MT * 16 * PW;
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < TREE_WARPS; ++w) M = fmaxf(M, p[w * ws + VHP]);
@@ -634,18 +640,44 @@ again:
       if (d < A.vh) acc += f * p[w * ws + d];
     }
     const int rr = r0 + r;
-    if (A.nsplit > 1) {
-      float* dst = A.part + ((((size_t)b * A.kvh + kh) * A.nsplit + z) * R + rr) * (A.vh + 2);
-      dst[d] = d < A.vh ? acc : d == A.vh ? M : L;
+    if (split) {
+      const float x = d < A.vh ? acc : d == A.vh ? M : L;
+      if (cluster)
+        P[TREE_WARPS * ws + (size_t)r * PW + d] = x;
+      else
+        A.part[((((size_t)b * A.kvh + kh) * A.nsplit + z) * R + rr) * (A.vh + 2) + d] = x;
     } else {
       const int n = A.by_rep.div(rr), h = kh * A.rep + rr - n * A.rep;
       A.out[(((size_t)b * A.T + n) * A.heads + h) * A.vh + d] = L == 0.f ? 0.f : acc / L;
     }
   }
+  if (!cluster) return;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  const float* own = P + TREE_WARPS * ws;
+  for (int i = tid; i < rows * A.vh; i += TREE_THREADS) {
+    const int r = i / A.vh, d = i - r * A.vh;
+    if (r % A.nsplit != z) continue;
+    float M = -INFINITY;
+    for (int s = 0; s < A.nsplit; ++s) M = fmaxf(M, cl.map_shared_rank(own, s)[(size_t)r * PW + A.vh]);
+    float L = 0.f, acc = 0.f;
+    for (int s = 0; s < A.nsplit; ++s) {
+      const float* p = cl.map_shared_rank(own, s) + (size_t)r * PW;
+      const float m = p[A.vh], l = p[A.vh + 1];
+      if (l == 0.f) continue;
+      const float f = m == -INFINITY ? 1.f : ex2(m - M);
+      L += f * l;
+      acc += f * p[d];
+    }
+    const int rr = r0 + r, n = A.by_rep.div(rr), h = kh * A.rep + rr - n * A.rep;
+    A.out[(((size_t)b * A.T + n) * A.heads + h) * A.vh + d] = L == 0.f ? 0.f : acc / L;
+  }
+  cl.sync();  // no block leaves while it may be read
 }
 
-// Joins the splits of one row per warp: weights 2^(m_z - M) in lanes, then
-// each lane sums its dimensions in split order.
+// Joins the splits, a warp a row: the weights 2^(m_z - M) in lanes, then two
+// neighbouring dims a lane, eight splits on their way at a time, in split order.
 __global__ void __launch_bounds__(256) tree_join_kernel(const float* __restrict__ part, int rows_all, int R, int T,
                                                         int heads, int kvh, int rep, int vh, int ns,
                                                         float* __restrict__ out) {
@@ -657,46 +689,70 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const float* __restrict_
   float M = -INFINITY;
   for (int z = lane; z < ns; z += 32) M = fmaxf(M, p[z * step + vh]);
   M = warp_max(M);
-  float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  float2 acc[2] = {{0.f, 0.f}, {0.f, 0.f}};
   for (int z0 = 0; z0 < ns; z0 += 32) {
     const int z = z0 + lane;
     float f = 0.f, l = 0.f;
     if (z < ns) {
-      const float m = p[z * step + vh];
-      l = p[z * step + vh + 1];
-      f = l == 0.f ? 0.f : m == -INFINITY ? 1.f : ex2(m - M);
+      const float2 ml = *reinterpret_cast<const float2*>(p + z * step + vh);
+      l = ml.y;
+      f = l == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : ex2(ml.x - M);  // a sum without a max is NaN, and stays
       l = l == 0.f ? 0.f : f * l;
     }
     L += warp_sum(l);
     const int n = min(32, ns - z0);
-    for (int i = 0; i < n; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      if (fi == 0.f) continue;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float2 x[8][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (lane + 32 * j < vh) acc[j] += fi * p[(z0 + i) * step + lane + 32 * j];
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = 2 * lane + 64 * j;
+          x[i][j] = i0 + i < n && d < vh ? *reinterpret_cast<const float2*>(p + (z0 + i0 + i) * step + d) : make_float2(0.f, 0.f);
+        }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float g = i0 + i < n ? __shfl_sync(0xffffffffu, f, i0 + i) : 0.f;
+        if (g == 0.f) continue;  // an empty split's row may hold anything
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[j].x += g * x[i][j].x, acc[j].y += g * x[i][j].y;
+      }
     }
   }
   const int t = r / rep, h = kh * rep + r - t * rep;
   float* dst = out + (((size_t)b * T + t) * heads + h) * vh;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (lane + 32 * j < vh) dst[lane + 32 * j] = L == 0.f ? 0.f : acc[j] / L;
+  for (int j = 0; j < 2; ++j) {
+    const int d = 2 * lane + 64 * j;
+    if (d < vh) dst[d] = L == 0.f ? 0.f : acc[j].x / L, dst[d + 1] = L == 0.f ? 0.f : acc[j].y / L;
+  }
 }
 
 template <bool I8, int QKP, int VHP, int MT>
 cudaError_t launch_tree(TreeArgs A, int B, int piece, cudaStream_t st) {
   using TT = TreeTile<I8, QKP, VHP>;
-  const size_t smem = std::max((size_t)TREE_WARPS * TT::WARP_BYTES, (size_t)TREE_WARPS * MT * 16 * (VHP + 4) * 4);
+  const size_t smem = std::max((size_t)TREE_WARPS * TT::WARP_BYTES, (size_t)(TREE_WARPS + 1) * MT * 16 * (VHP + 4) * 4);
   auto kern = attend_tree_kernel<I8, QKP, VHP, MT>;
-  cudaError_t e = allow_smem((const void*)kern, smem);
+  cudaError_t e = allow_smem((const void*)kern, smem, true);
   if (e != cudaSuccess) return e;
   const int R = A.T * A.rep, tiles = (R + MT * 16 - 1) / (MT * 16);
+  const int cluster = A.nsplit > 1 && !A.part;
   for (int b0 = 0; b0 < B; b0 += 65535) {
     const int n = std::min(65535, B - b0);
     const TreeArgs C = tree_sessions(A, b0, TT::ES);
-    kern<<<dim3((unsigned)tiles * A.kvh * A.nsplit, n), TREE_THREADS, smem, st>>>(C, piece);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles * A.kvh * A.nsplit, n);
+    cfg.blockDim = dim3(TREE_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster ? A.nsplit : 1;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kern, C, piece, cluster);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -718,12 +774,16 @@ TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv,
   P.umma = al16(out) && tree_umma_takes(int8, R, qk, vh, P.piece);
   if (P.umma) {
     P.nsplit = tree_umma_nsplit(B, R, kvh, qk, vh, slots + (tk ? T : 0));
+    P.part = P.nsplit > 1;
     return P;
   }
   const int tr = tree_tile_rows(R, qk, vh);
   const long ctas = (long)B * kvh * ((R + tr - 1) / tr);
   const long want = (592 + ctas - 1) / ctas, most = std::max(1, (slots + 255) / 256);
   P.nsplit = (int)std::max(1l, std::min(std::min(want, most), 256l));
+  // Up to eight splits are a cluster that joins itself; more leave partial
+  // results for a second kernel.
+  P.part = P.nsplit > TREE_CLUSTER;
   return P;
 }
 
@@ -759,7 +819,7 @@ cudaError_t launch_attend_tree(const float* q, int ldq, const void* k, const voi
   else if (one) NB_TREE(48, 64, 1);
   else NB_TREE(48, 64, 2);
 #undef NB_TREE
-  if (e != cudaSuccess || plan.nsplit == 1) return e;
+  if (e != cudaSuccess || !plan.part) return e;
   const long rows = (long)B * T * heads;
   tree_join_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(part, (int)rows, R, T, heads, kvh, A.rep, vh, plan.nsplit,
                                                                out);

@@ -1024,7 +1024,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
 template <class C>
 cudaError_t launch_umma_form(const TreeArgs& A, int B, cudaStream_t st) {
   auto kern = tree_umma_kernel<C>;
-  cudaError_t e = allow_smem((const void*)kern, C::SMEM);
+  cudaError_t e = allow_smem((const void*)kern, C::SMEM, true);
   if (e != cudaSuccess) return e;
   // The warpgroups' register shares assume the launch's: another count would
   // leave setmaxnreg waiting.
