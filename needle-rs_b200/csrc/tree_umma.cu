@@ -49,7 +49,7 @@ struct TreeUmma {
   static constexpr int THREADS = 2 * W * 128, CTAS = W == 1 ? 2 : 1;
   // Registers a thread: the launch's, a softmax thread's, the other warpgroup's;
   // the warpgroups' shares add up to the launch's.
-  static constexpr int REG_ALL = 128, REG_SOFT = W == 1 ? (I8 ? 184 : 176) : 192, REG_PROD = 256 - REG_SOFT;
+  static constexpr int REG_ALL = 128, REG_SOFT = W == 1 ? (I8 ? 184 : 160) : 208, REG_PROD = 256 - REG_SOFT;
   static constexpr int WG_COLS = 2 * BN + VP;     // TMEM columns of a warpgroup: two of S (then P), O
   static constexpr int TMEM = W * WG_COLS <= 128 ? 128 : W * WG_COLS <= 256 ? 256 : 512;
   static constexpr size_t META = NST * (size_t)(BN * 8 + 16 + 16) + 128 * 4 + 512;
@@ -428,78 +428,56 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         // them in registers; 128-wide ones, whose outputs fill the registers,
         // read S twice.
         constexpr bool KEEP = VP == 64;
-        f32x2 s[KEEP ? 32 : 16];
+        f32x2 s[KEEP ? 32 : 8];
         float mx = -INFINITY;
-        auto scores = [&](const uint32_t (&x)[32], int c, f32x2* to) {  // half c of the sub-block
+        auto scores = [&](const uint32_t (&x)[16], int c, f32x2* to) {  // positions 16 c .. + 15
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 k = k4[c * 8 + j];
+          for (int j = 0; j < 4; ++j) {
+            const float4 k = k4[c * 4 + j];
             to[2 * j] = mul2(pk(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1])), pk(k.x, k.y));
             to[2 * j + 1] = mul2(pk(__uint_as_float(x[4 * j + 2]), __uint_as_float(x[4 * j + 3])), pk(k.z, k.w));
           }
           if (!all) {
+            const uint32_t w = sees[c >> 1] >> ((c & 1) * 16);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < 8; ++j) {
               float f0, f1;
               up(to[j], f0, f1);
-              to[j] = pk((sees[c] >> (2 * j)) & 1 ? f0 : -INFINITY, (sees[c] >> (2 * j + 1)) & 1 ? f1 : -INFINITY);
+              to[j] = pk((w >> (2 * j)) & 1 ? f0 : -INFINITY, (w >> (2 * j + 1)) & 1 ? f1 : -INFINITY);
             }
           }
         };
         auto top_of = [&](const f32x2* a) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
+          for (int j = 0; j < 8; ++j) {
             float f0, f1;
             up(a[j], f0, f1);
             mx = fmaxf(fmaxf(mx, f0), f1);
           }
         };
         if (KEEP) {
-          uint32_t x0[32], x1[32];
-          tmem_ld32(s_now, x0);
-          tmem_ld32(s_now + 32, x1);
+          uint32_t x[4][16];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld16(s_now + 16 * c, x[c]);
           tmem_landed();
-          scores(x0, 0, s);
-          scores(x1, 1, s + (KEEP ? 16 : 0));
-          top_of(s);
-          top_of(s + (KEEP ? 16 : 0));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) scores(x[c], c, s + (KEEP ? 8 * c : 0));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) top_of(s + (KEEP ? 8 * c : 0));
         } else {
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t x[32];
-            tmem_ld32(s_now + 32 * c, x);
+          uint32_t x[2][16];
+          tmem_ld16(s_now, x[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
             tmem_landed();
-            scores(x, c, s);
+            if (c < 3) tmem_ld16(s_now + 16 * (c + 1), x[(c + 1) & 1]);
+            scores(x[c & 1], c, s);
             top_of(s);
           }
         }
         const float mn = fmaxf(m, mx * qs), mz = mn == -INFINITY ? 0.f : mn;
         const float corr = ex2(m - mz);
         m = mn;
-        // ---- the last sub-block's output, then the new scale
-        const int e = expo[2 * st];
-        low = expo[2 * st + 1];
-        if (it > 0) {
-          if (!mbar_wait_asleep(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
-          ok = __all_sync(0xffffffffu, ok);
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < VP; c += 32) {
-            uint32_t x[2][16];
-            tmem_ld16(o_at + lanes + c, x[0]);
-            tmem_ld16(o_at + lanes + c + 16, x[1]);
-            tmem_landed();
-#pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              o[(c + j) / 2] = add2(o[(c + j) / 2], pk(__uint_as_float(x[j >> 4][j & 15]), __uint_as_float(x[j >> 4][(j & 15) + 1])));
-          }
-          const float by = corr * (e - e_old > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (e - e_old)) << 23));
-          if (__any_sync(0xffffffffu, by != 1.f)) {
-#pragma unroll
-            for (int d = 0; d < VP / 2; ++d) o[d] = mul2(o[d], pk(by, by));
-          }
-        }
-        e_old = e;
         // ---- weights: sum, and times the value scale as f16 parts into S's place
         // (16 positions' columns take 8 of high parts, then 8 of remainders)
         f32x2 add = pk(0.f, 0.f);
@@ -530,19 +508,44 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
 #pragma unroll
           for (int c = 0; c < 4; ++c) weights(s + (KEEP ? c * 8 : 0), c);
         } else {
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
-            uint32_t x[32];
-            tmem_ld32(s_now + 32 * c, x);
+          // A chunk's columns are overwritten by its own weights only.
+          uint32_t x[2][16];
+          tmem_ld16(s_now, x[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
             tmem_landed();
-            scores(x, c, s);
-            weights(s, 2 * c);
-            weights(s + 8, 2 * c + 1);
+            if (c < 3) tmem_ld16(s_now + 16 * (c + 1), x[(c + 1) & 1]);
+            scores(x[c & 1], c, s);
+            weights(s, c);
           }
         }
         float a, d;
         up(add, a, d);
         l = l * corr + (a + d);
+        // ---- the last step's output (its product ran under the weights), then the new scale
+        const int e = expo[2 * st];
+        low = expo[2 * st + 1];
+        if (it > 0) {
+          if (!mbar_wait_asleep(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < VP; c += 32) {
+            uint32_t x[2][16];
+            tmem_ld16(o_at + lanes + c, x[0]);
+            tmem_ld16(o_at + lanes + c + 16, x[1]);
+            tmem_landed();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              o[(c + j) / 2] = add2(o[(c + j) / 2], pk(__uint_as_float(x[j >> 4][j & 15]), __uint_as_float(x[j >> 4][(j & 15) + 1])));
+          }
+          const float by = corr * (e - e_old > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (e - e_old)) << 23));
+          if (__any_sync(0xffffffffu, by != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < VP / 2; ++d) o[d] = mul2(o[d], pk(by, by));
+          }
+        }
+        e_old = e;
         tmem_wait_st();
         tc_fence_before();
       }
@@ -802,28 +805,27 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
             const bool in = v < P.total;
             const float4* src = reinterpret_cast<const float4*>(
                 reinterpret_cast<const float*>(P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk);
-            // Twice over the row (the second time from cache): its largest element, then its parts.
+            float4 x[QS * 4];
+#pragma unroll
+            for (int c = 0; c < QS * 4; ++c) x[c] = in && c * 4 < A.qk ? __ldg(src + c) : make_float4(0, 0, 0, 0);
             float mx = 0.f;
             bool fine = true;
-#pragma unroll 4
+#pragma unroll
             for (int c = 0; c < QS * 4; ++c) {
-              const float4 f = in && c * 4 < A.qk ? __ldg(src + c) : make_float4(0, 0, 0, 0);
-              const float a = fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w)));
-              const float t = fabsf(f.x) + fabsf(f.y) + fabsf(f.z) + fabsf(f.w);  // NaN where one is
+              const float a = fmaxf(fmaxf(fabsf(x[c].x), fabsf(x[c].y)), fmaxf(fabsf(x[c].z), fabsf(x[c].w)));
+              const float t = fabsf(x[c].x) + fabsf(x[c].y) + fabsf(x[c].z) + fabsf(x[c].w);  // NaN where one is
               fine &= a <= 3.4028234e38f && t == t;
               mx = fmaxf(mx, a);
             }
             const int ef = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
             const float by = __uint_as_float((uint32_t)(267 - ef) << 23);
-#pragma unroll 2
+#pragma unroll
             for (int c = 0; c < QS * 2; ++c) {
-              const float4 f = in && c * 8 < A.qk ? __ldg(src + 2 * c) : make_float4(0, 0, 0, 0);
-              const float4 g = in && c * 8 < A.qk ? __ldg(src + 2 * c + 1) : make_float4(0, 0, 0, 0);
               uint32_t hh[4], ll[4];
-              halves(f.x * by, f.y * by, &hh[0], &ll[0]);
-              halves(f.z * by, f.w * by, &hh[1], &ll[1]);
-              halves(g.x * by, g.y * by, &hh[2], &ll[2]);
-              halves(g.z * by, g.w * by, &hh[3], &ll[3]);
+              halves(x[2 * c].x * by, x[2 * c].y * by, &hh[0], &ll[0]);
+              halves(x[2 * c].z * by, x[2 * c].w * by, &hh[1], &ll[1]);
+              halves(x[2 * c + 1].x * by, x[2 * c + 1].y * by, &hh[2], &ll[2]);
+              halves(x[2 * c + 1].z * by, x[2 * c + 1].w * by, &hh[3], &ll[3]);
               unsigned char* at = kt + kp * 128 + ((c ^ (kp & 7)) << 4);
               *reinterpret_cast<uint4*>(at) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
               *reinterpret_cast<uint4*>(at + C::K_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
@@ -919,14 +921,18 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           auto at = [&](const float* row, int d) {
             return row && d < A.vh ? __ldg(reinterpret_cast<const float4*>(row + d)) : make_float4(0, 0, 0, 0);
           };
-          // Twice over the values (the second time from cache): exponent field of
-          // each position's largest (0 none, 255 not finite), then the parts.
-          int top = 0, least = 255;
-          uint32_t ef[2] = {0, 0}, bad = 0;  // a byte a position
-#pragma unroll 2
+          float4 x[2][8];
+#pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float* row = row_of(j);
-            const float4 f = at(row, (lane >> 2) * 4), g = at(row, 32 + (lane >> 2) * 4);
+            x[0][j] = at(row, (lane >> 2) * 4), x[1][j] = at(row, 32 + (lane >> 2) * 4);
+          }
+          // Exponent field of each position's largest value (0 none, 255 not finite), a byte a position.
+          int top = 0, least = 255;
+          uint32_t ef[2] = {0, 0}, bad = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 f = x[0][j], g = x[1][j];
             float a = fmaxf(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))),
                             fmaxf(fmaxf(fabsf(g.x), fabsf(g.y)), fmaxf(fabsf(g.z), fabsf(g.w))));
             const float t = fabsf(f.x) + fabsf(f.y) + fabsf(f.z) + fabsf(f.w) + fabsf(g.x) + fabsf(g.y) + fabsf(g.z) +
@@ -934,10 +940,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
             if (t != t) a = INFINITY;
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-            const int x = a == 0.f ? 0 : a <= 3.4028234e38f ? min(max((int)(__float_as_uint(a) >> 23), 14), 253) : 255;
-            if (x == 255) bad |= 1u << (8 * oc + j);
-            else if (x > 0) top = max(top, x - 13), least = min(least, x - 13);
-            ef[j >> 2] |= (uint32_t)x << (8 * (j & 3));
+            const int y = a == 0.f ? 0 : a <= 3.4028234e38f ? min(max((int)(__float_as_uint(a) >> 23), 14), 253) : 255;
+            if (y == 255) bad |= 1u << (8 * oc + j);
+            else if (y > 0) top = max(top, y - 13), least = min(least, y - 13);
+            ef[j >> 2] |= (uint32_t)y << (8 * (j & 3));
           }
           top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
           bad = __reduce_or_sync(0xffffffffu, bad);
@@ -956,17 +962,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               col_v[st * BN + pr * 8 + j] = x > 0 && x < 255 && f > 0 ? __uint_as_float((uint32_t)f << 23) : 0.f;
             }
           }
-#pragma unroll 1
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int d0 = h * 32 + (lane >> 2) * 4;
-            float4 x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int y = (int)((ef[j >> 2] >> (8 * (j & 3))) & 255u);
               const bool use = y > 0 && y < 255;  // nothing of one that is not finite
-              const float by = use ? __uint_as_float((uint32_t)(267 - y) << 23) : 0.f;
-              x[j] = at(use ? row_of(j) : nullptr, d0);
-              x[j].x *= by, x[j].y *= by, x[j].z *= by, x[j].w *= by;
+              const float by = __uint_as_float((uint32_t)(267 - (use ? y : 140)) << 23);
+              x[h][j].x = use ? x[h][j].x * by : 0.f, x[h][j].y = use ? x[h][j].y * by : 0.f;
+              x[h][j].z = use ? x[h][j].z * by : 0.f, x[h][j].w = use ? x[h][j].w * by : 0.f;
             }
             if (d0 >= A.vh) continue;
 #pragma unroll
@@ -974,7 +979,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               uint32_t hh[4], ll[4];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float4 a = x[2 * j], c = x[2 * j + 1];
+                const float4 a = x[h][2 * j], c = x[h][2 * j + 1];
                 halves(t == 0 ? a.x : t == 1 ? a.y : t == 2 ? a.z : a.w, t == 0 ? c.x : t == 1 ? c.y : t == 2 ? c.z : c.w,
                        &hh[j], &ll[j]);
               }
