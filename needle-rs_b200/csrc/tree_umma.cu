@@ -13,16 +13,18 @@
 // and truncation costs only what the sum already holds. For the same reason O
 // is drained into f32 registers after every block.
 //
-// Warps: W softmax warpgroups (step i belongs to warpgroup i % W, each with its
-// own running max, sum and output, merged at the end), and for each another one of
+// Warps: one softmax warpgroup with a thread a row, or, for 128-wide heads,
+// whose outputs would fill a thread's registers, two with half of a row's
+// positions and half of its outputs each (they tell each other their maxima),
+// and one warpgroup of
 //   a key warp and two value warps, which read the ring and the draft, widen
 //   them to f16 and lay them down in the 128-byte swizzled form the MMA reads
 //   (keys as they lie, values transposed eight positions at a time in
 //   registers; the key warp also forms the steps' scales), and
 //   an MMA warp, which issues every product as soon as its operands stand: a
 //   warp that issues MMAs is held for as long as they run.
-// With W = 1 two blocks share an SM and hide each other's latencies; 128-wide
-// heads need the shared memory of a whole SM and W = 2.
+// Heads of up to 64 leave room for two blocks on an SM, which hide each other's
+// latencies; 128-wide heads need the shared memory of a whole SM.
 //
 // Every wait is bounded as in umma_gemm.cu.
 #include <algorithm>
@@ -35,24 +37,27 @@
 namespace nb {
 namespace {
 
-template <bool I8_, int QS_, int VP_, int W_, int NST_>
+template <bool I8_, int QS_, int VP_, int NST_>
 struct TreeUmma {
   static constexpr bool I8 = I8_;
-  static constexpr int QS = QS_;    // k16 steps of the key product
-  static constexpr int VP = VP_;    // value width held (64 or 128)
-  static constexpr int W = W_, NST = NST_;
-  static constexpr int BN = 64;                   // positions of a stage, and of a step of the softmax
+  static constexpr int QS = QS_;        // k16 steps of the key product
+  static constexpr int VP = VP_;        // value width held (64 or 128)
+  static constexpr int TPR = VP / 64;   // softmax threads a row
+  static constexpr int NST = NST_;
+  static constexpr int BN = 64;         // positions of a stage, and of a step of the softmax
+  static constexpr int CW = BN / TPR;   // positions of a softmax thread's step
   static constexpr int KA = (QS * 16 + 63) / 64;  // 64-wide swizzle atoms of a key row
   static constexpr int PARTS = I8 ? 1 : 2;        // high part, remainder
   static constexpr int Q_TILE = KA * 128 * 128, K_TILE = KA * BN * 128, V_TILE = VP * 128;
   static constexpr int STAGE = PARTS * (K_TILE + V_TILE);
-  static constexpr int THREADS = 2 * W * 128, CTAS = W == 1 ? 2 : 1;
+  static constexpr int THREADS = (TPR + 1) * 128, CTAS = TPR == 1 ? 2 : 1;
   // Registers a thread: the launch's, a softmax thread's, the other warpgroup's;
   // the warpgroups' shares add up to the launch's.
-  static constexpr int REG_ALL = 128, REG_SOFT = W == 1 ? (I8 ? 184 : 160) : 208, REG_PROD = 256 - REG_SOFT;
-  static constexpr int WG_COLS = 2 * BN + VP;     // TMEM columns of a warpgroup: two of S (then P), O
-  static constexpr int TMEM = W * WG_COLS <= 128 ? 128 : W * WG_COLS <= 256 ? 256 : 512;
-  static constexpr size_t META = NST * (size_t)(BN * 8 + 16 + 16) + 128 * 4 + 512;
+  static constexpr int REG_ALL = TPR == 1 ? 128 : 168, REG_SOFT = TPR == 1 ? (I8 ? 184 : 160) : 176,
+                       REG_PROD = (TPR + 1) * REG_ALL - TPR * REG_SOFT;
+  static_assert(TPR * REG_SOFT + REG_PROD == (TPR + 1) * REG_ALL && REG_PROD % 8 == 0, "register shares");
+  static constexpr int TMEM = 2 * BN + VP <= 128 ? 128 : 256;  // columns: two of S (then P), O
+  static constexpr size_t META = NST * (size_t)(BN * 8 + 16 + 16) + 128 * 4 + 512 + 2 * 2 * 128 * 4;
   static constexpr size_t SMEM = 1024 + 2 * (size_t)Q_TILE + NST * (size_t)STAGE + META;
 };
 
@@ -85,16 +90,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(tree_idesc<N>()), "r"(accum));
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(t));
-}
 // One lane of a converged warp, in a form the compiler knows to be uniform.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -247,7 +242,7 @@ __device__ __noinline__ void tree_slow_row(const TreeArgs& A, const TreePlace& P
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __grid_constant__ TreeArgs A, int* werr) {
   constexpr bool I8 = C::I8;
-  constexpr int BN = C::BN, VP = C::VP, QS = C::QS, W = C::W, NST = C::NST, NC = BN / 32;
+  constexpr int BN = C::BN, VP = C::VP, QS = C::QS, TPR = C::TPR, CW = C::CW, NST = C::NST, NC = BN / 32;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   unsigned char *qhi = sm, *qlo = sm + C::Q_TILE, *stages = sm + 2 * C::Q_TILE;
@@ -258,16 +253,17 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
   float* row_q = reinterpret_cast<float*>(expo + 2 * NST);                  // [128] score scale of a row
   uint64_t* full = reinterpret_cast<uint64_t*>(row_q + 128);
   uint64_t* empty = full + NST;
-  uint64_t* s_full = empty + NST;   // [W][2] S of the warpgroup's sub-block
-  uint64_t* o_full = s_full + 2 * W;  // [W] O of the warpgroup's sub-block
-  uint64_t* p_full = o_full + W;    // [W] P of the warpgroup's step, one arrival a warp with rows
-  uint64_t* q_full = p_full + W;    // the queries
-  uint64_t* drain = q_full + 1;     // every MMA
+  uint64_t* s_full = empty + NST;  // [2] S of a step
+  uint64_t* o_full = s_full + 2;   // O of a step
+  uint64_t* p_full = o_full + 1;   // P of a step, one arrival a softmax warp with rows
+  uint64_t* q_full = p_full + 1;   // the queries
+  uint64_t* drain = q_full + 1;    // every MMA
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile uint32_t* abort = tmem_slot + 1;
   int* range = reinterpret_cast<int*>(tmem_slot + 2);    // [2]
   uint32_t* slow = reinterpret_cast<uint32_t*>(range + 2);  // [4] rows for tree_slow_row
   int* vmax = reinterpret_cast<int*>(slow + 4);             // [2][4] the value warps' exponents
+  float* both = reinterpret_cast<float*>(full) + 128;       // [2][2][128] what two threads of a row tell each other
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int b = blockIdx.y;
@@ -283,12 +279,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       mbar_init(&full[s], 96);   // the key and value warps
       mbar_init(&empty[s], 1);   // one tcgen05.commit
     }
-    for (int w = 0; w < W; ++w) {
-      mbar_init(&s_full[2 * w], 1);
-      mbar_init(&s_full[2 * w + 1], 1);
-      mbar_init(&o_full[w], 1);
-      mbar_init(&p_full[w], (rows + 31) / 32);
-    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(o_full, 1);
+    mbar_init(p_full, TPR * ((rows + 31) / 32));
     mbar_init(q_full, 128);
     mbar_init(drain, 1);
     *abort = 0;
@@ -344,11 +338,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
   }
 
   const int wg = warp >> 2;
-  if (wg < W) {
+  if (wg < TPR) {
     // ------------------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFT));
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + wg * C::WG_COLS, o_at = s_at + 128;
+    const uint32_t s_at = tmem + wg * CW, o_at = tmem + 2 * BN + wg * 64;  // the thread's columns of S and O
     // ---- queries: a row a thread of the first warpgroup, scaled by the power
     // of two that brings the row's max into [2^13, 2^14)
     if (wg == 0) {
@@ -383,7 +377,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(q_full);
     }
-    if (W == 2) asm volatile("bar.sync 3, 256;" ::: "memory");
+    if (TPR == 2) asm volatile("bar.sync 5, 256;" ::: "memory");
     const float qs = row_q[r];
     // Positions every row of the warp sees without a look at the mask.
     int full0 = A.drafted + start, full1 = A.drafted + min(start + cnt, n_ring);
@@ -392,89 +386,80 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       full0 = max(full0, __shfl_xor_sync(0xffffffffu, full0, d));
       full1 = min(full1, __shfl_xor_sync(0xffffffffu, full1, d));
     }
-    f32x2 o[VP / 2];  // dims 2 d, 2 d + 1
+    f32x2 o[32];  // dims 2 d, 2 d + 1 of the thread's 64
     float m = -INFINITY, l = 0.f;
     bool is_slow = false, ok = true;
 #pragma unroll
-    for (int d = 0; d < VP / 2; ++d) o[d] = pk(0.f, 0.f);
-    // Step jj of the warpgroup takes stage i = jj W + wg. Warps whose rows are
-    // all padding take no part.
-    const int nj = (warp & 3) * 32 < rows && nblk > wg ? (nblk - wg + W - 1) / W : 0;
+    for (int d = 0; d < 32; ++d) o[d] = pk(0.f, 0.f);
+    // Warps whose rows are all padding take no part.
+    const int nj = (warp & 3) * 32 < rows ? nblk : 0;
+    // What a thread has for the other of its row, and has from it; `turn`
+    // alternates between two places, so one meeting a turn is enough.
+    auto meet = [&](int turn, float mine_) {
+      both[turn * 256 + wg * 128 + r] = mine_;
+      if ((warp & 3) == 0) asm volatile("bar.sync 1, 64;" ::: "memory");
+      else if ((warp & 3) == 1) asm volatile("bar.sync 2, 64;" ::: "memory");
+      else if ((warp & 3) == 2) asm volatile("bar.sync 3, 64;" ::: "memory");
+      else asm volatile("bar.sync 6, 64;" ::: "memory");
+      return both[turn * 256 + (1 - wg) * 128 + r];
+    };
 
-    int e_old = 14, it = 0;
+    int e_old = 14;
     int low = 255;
-    for (int jj = 0; jj < nj; ++jj, ++it) {
-      const int i = jj * W + wg, st = i % NST;
-      if (ok && !mbar_wait_asleep(&s_full[2 * wg + (jj & 1)], (uint32_t)(jj >> 1) & 1u, abort, werr)) ok = false;
+    for (int i = 0; i < nj; ++i) {
+      const int st = i % NST;
+      if (ok && !mbar_wait_asleep(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, abort, werr)) ok = false;
       if (ok && !mbar_wait_asleep(&full[st], (uint32_t)(i / NST) & 1u, abort, werr)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
+      float mx = -INFINITY;
+      f32x2 s[CW / 2];
+      const uint32_t s_now = s_at + lanes + (i & 1) * BN;
+      const float4* v4 = reinterpret_cast<const float4*>(col_v + st * BN + wg * CW);
       if (ok) {
         tc_fence_after();
-        const int v0 = (blk0 + i) * BN;
-        const uint32_t s_now = s_at + lanes + (jj & 1) * BN;
-        const float4* k4 = reinterpret_cast<const float4*>(col_k + st * BN);
-        const float4* v4 = reinterpret_cast<const float4*>(col_v + st * BN);
-        const bool all = v0 >= full0 && v0 + BN <= full1;  // the same for the warp
-        uint32_t sees[2] = {0xffffffffu, 0xffffffffu};
-        if (!all) {
+        const int v0 = (blk0 + i) * BN + wg * CW;
+        const float4* k4 = reinterpret_cast<const float4*>(col_k + st * BN + wg * CW);
+        const bool all = v0 >= full0 && v0 + CW <= full1;  // the same for the warp
+        uint32_t sees[CW / 32];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) sees[c] = mine ? tree_sees(A, node_at, node, start, cnt, n_ring, v0 + 32 * c) : 0u;
+        for (int c = 0; c < CW / 32; ++c) {
+          sees[c] = 0xffffffffu;
+          if (!all) sees[c] = mine ? tree_sees(A, node_at, node, start, cnt, n_ring, v0 + 32 * c) : 0u;
+          const int w = wg * (CW / 32) + c;
+          is_slow |= (sees[c] & (I8 ? odd[st * NC + w] : odd[st * 2 * NC + w] | odd[st * 2 * NC + NC + w])) != 0;
         }
-        if (I8)
-          is_slow |= ((sees[0] & odd[st * NC]) | (sees[1] & odd[st * NC + 1])) != 0;
-        else
-          is_slow |= ((sees[0] & (odd[st * 4] | odd[st * 4 + 2])) | (sees[1] & (odd[st * 4 + 1] | odd[st * 4 + 3]))) != 0;
-        // ---- scores times the key scales, and their max. 64-wide heads keep
-        // them in registers; 128-wide ones, whose outputs fill the registers,
-        // read S twice.
-        constexpr bool KEEP = VP == 64;
-        f32x2 s[KEEP ? 32 : 8];
-        float mx = -INFINITY;
-        auto scores = [&](const uint32_t (&x)[16], int c, f32x2* to) {  // positions 16 c .. + 15
+        // ---- scores times the key scales, and their max
+        uint32_t x[CW / 16][16];
+#pragma unroll
+        for (int c = 0; c < CW / 16; ++c) tmem_ld16(s_now + 16 * c, x[c]);
+        tmem_landed();
+#pragma unroll
+        for (int c = 0; c < CW / 16; ++c)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float4 k = k4[c * 4 + j];
-            to[2 * j] = mul2(pk(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1])), pk(k.x, k.y));
-            to[2 * j + 1] = mul2(pk(__uint_as_float(x[4 * j + 2]), __uint_as_float(x[4 * j + 3])), pk(k.z, k.w));
+            s[8 * c + 2 * j] = mul2(pk(__uint_as_float(x[c][4 * j]), __uint_as_float(x[c][4 * j + 1])), pk(k.x, k.y));
+            s[8 * c + 2 * j + 1] =
+                mul2(pk(__uint_as_float(x[c][4 * j + 2]), __uint_as_float(x[c][4 * j + 3])), pk(k.z, k.w));
           }
-          if (!all) {
-            const uint32_t w = sees[c >> 1] >> ((c & 1) * 16);
+        if (!all) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              float f0, f1;
-              up(to[j], f0, f1);
-              to[j] = pk((w >> (2 * j)) & 1 ? f0 : -INFINITY, (w >> (2 * j + 1)) & 1 ? f1 : -INFINITY);
-            }
-          }
-        };
-        auto top_of = [&](const f32x2* a) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < CW / 2; ++j) {
+            const uint32_t w = sees[j >> 4] >> (2 * (j & 15));
             float f0, f1;
-            up(a[j], f0, f1);
-            mx = fmaxf(fmaxf(mx, f0), f1);
-          }
-        };
-        if (KEEP) {
-          uint32_t x[4][16];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld16(s_now + 16 * c, x[c]);
-          tmem_landed();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) scores(x[c], c, s + (KEEP ? 8 * c : 0));
-#pragma unroll
-          for (int c = 0; c < 4; ++c) top_of(s + (KEEP ? 8 * c : 0));
-        } else {
-          uint32_t x[2][16];
-          tmem_ld16(s_now, x[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_landed();
-            if (c < 3) tmem_ld16(s_now + 16 * (c + 1), x[(c + 1) & 1]);
-            scores(x[c & 1], c, s);
-            top_of(s);
+            up(s[j], f0, f1);
+            s[j] = pk(w & 1 ? f0 : -INFINITY, w & 2 ? f1 : -INFINITY);
           }
         }
+#pragma unroll
+        for (int j = 0; j < CW / 2; ++j) {
+          float f0, f1;
+          up(s[j], f0, f1);
+          mx = fmaxf(fmaxf(mx, f0), f1);
+        }
+      }
+      if (TPR == 2) mx = fmaxf(mx, meet(i & 1, mx));
+      if (ok) {
         const float mn = fmaxf(m, mx * qs), mz = mn == -INFINITY ? 0.f : mn;
         const float corr = ex2(m - mz);
         m = mn;
@@ -482,7 +467,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         // (16 positions' columns take 8 of high parts, then 8 of remainders)
         f32x2 add = pk(0.f, 0.f);
         const f32x2 qs2 = pk(qs, qs), mz2 = pk(-mz, -mz);
-        auto weights = [&](const f32x2* a, int c) {  // 16 positions from 16 c
+#pragma unroll
+        for (int c = 0; c < CW / 16; ++c) {
           uint32_t hi[8], lo[8];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -490,11 +476,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               float f0, f1, w0, w1;
-              up(fma2(a[2 * j + g], qs2, mz2), f0, f1);
+              up(fma2(s[8 * c + 2 * j + g], qs2, mz2), f0, f1);
               const f32x2 p = pk(ex2(f0), ex2(f1));
               add = add2(add, p);
-              const f32x2 w = mul2(p, g ? pk(vv.z, vv.w) : pk(vv.x, vv.y));
-              up(w, w0, w1);
+              up(mul2(p, g ? pk(vv.z, vv.w) : pk(vv.x, vv.y)), w0, w1);
               const float t0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u),
                           t1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
               hi[2 * j + g] = cvt2(t0, t1);
@@ -503,21 +488,6 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           }
           tmem_st8(s_now + c * 16, hi);
           tmem_st8(s_now + c * 16 + 8, lo);
-        };
-        if (KEEP) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) weights(s + (KEEP ? c * 8 : 0), c);
-        } else {
-          // A chunk's columns are overwritten by its own weights only.
-          uint32_t x[2][16];
-          tmem_ld16(s_now, x[0]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_landed();
-            if (c < 3) tmem_ld16(s_now + 16 * (c + 1), x[(c + 1) & 1]);
-            scores(x[c & 1], c, s);
-            weights(s, c);
-          }
         }
         float a, d;
         up(add, a, d);
@@ -525,12 +495,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         // ---- the last step's output (its product ran under the weights), then the new scale
         const int e = expo[2 * st];
         low = expo[2 * st + 1];
-        if (it > 0) {
-          if (!mbar_wait_asleep(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
+        if (i > 0) {
+          if (!mbar_wait_asleep(o_full, (uint32_t)(i - 1) & 1u, abort, werr)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < VP; c += 32) {
+          for (int c = 0; c < 64; c += 32) {
             uint32_t x[2][16];
             tmem_ld16(o_at + lanes + c, x[0]);
             tmem_ld16(o_at + lanes + c + 16, x[1]);
@@ -542,7 +512,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           const float by = corr * (e - e_old > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (e - e_old)) << 23));
           if (__any_sync(0xffffffffu, by != 1.f)) {
 #pragma unroll
-            for (int d = 0; d < VP / 2; ++d) o[d] = mul2(o[d], pk(by, by));
+            for (int d2 = 0; d2 < 32; ++d2) o[d2] = mul2(o[d2], pk(by, by));
           }
         }
         e_old = e;
@@ -550,26 +520,27 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         tc_fence_before();
       }
       __syncwarp();
-      if (ok && lane == 0) mbar_arrive(&p_full[wg]);
+      if (ok && lane == 0) mbar_arrive(p_full);
     }
-    if (it > 0) {
-      if (ok && !mbar_wait_asleep(&o_full[wg], (uint32_t)(it - 1) & 1u, abort, werr)) ok = false;
+    if (nj > 0) {
+      float top = 0.f;
+      bool faint = false;
+      if (ok && !mbar_wait_asleep(o_full, (uint32_t)(nj - 1) & 1u, abort, werr)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
         // Outputs to their own scale. A row whose output came out infinite or
-        // NaN, or far below what the block's largest value scale holds bits
-        // for, is done again.
+        // NaN, or far below what the largest value scale holds bits for, is done
+        // again.
         const float by = __uint_as_float((uint32_t)(e_old - 13) << 23);
-        float top = 0.f;
         bool bad = false;
 #pragma unroll
-        for (int c = 0; c < VP; c += 32) {
-          uint32_t x[32];
-          tmem_ld32(o_at + lanes + c, x);
-          tmem_wait_ld();
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t x[16];
+          tmem_ld16(o_at + lanes + c, x);
+          tmem_landed();
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
+          for (int j = 0; j < 16; j += 2) {
             const f32x2 t = add2(o[(c + j) / 2], pk(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
             float t0, t1;
             up(t, t0, t1);
@@ -578,74 +549,49 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
             o[(c + j) / 2] = mul2(t, pk(by, by));
           }
         }
-        is_slow |= bad || (e_old - low > 12 && l > 0.f && top < (I8 ? 2.f : 16384.f) * l);
+        is_slow |= bad;
+        faint = e_old - low > 12;
       } else {  // a wait gave up: the flag is up, and the rows say so
 #pragma unroll
-        for (int d = 0; d < VP / 2; ++d) o[d] = pk(__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u));
+        for (int d = 0; d < 32; ++d) o[d] = pk(__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u));
         l = 1.f, m = 0.f;
         is_slow = false;
       }
+      if (TPR == 2) l += meet(nj & 1, l);
+      is_slow |= faint && l > 0.f && top < (I8 ? 2.f : 16384.f) * l;
+      if (mine && is_slow) atomicOr(&slow[r >> 5], 1u << (r & 31));
+      if (TPR == 2) is_slow |= meet(~nj & 1, is_slow ? 1.f : 0.f) != 0.f;
     }
-    if (mine && is_slow) atomicOr(&slow[r >> 5], 1u << (r & 31));
-    // ---- merge the warpgroups (every block is consumed: the stages' memory is
-    // free) and write
-    if (W == 2) {
-      // [VP / 2][128] pairs, then [2][128] max and sum
-      f32x2* xch = reinterpret_cast<f32x2*>(stages);
-      float* xml = reinterpret_cast<float*>(xch + VP / 2 * 128);
-      asm volatile("bar.sync 3, 256;" ::: "memory");
-      if (wg == 1) {
-#pragma unroll
-        for (int d = 0; d < VP / 2; ++d) xch[d * 128 + r] = o[d];
-        xml[r] = m, xml[128 + r] = l;
-      }
-      asm volatile("bar.sync 3, 256;" ::: "memory");
-      is_slow = (slow[r >> 5] >> (r & 31)) & 1;
-      if (wg == 0) {
-        const float m1 = xml[r], l1 = xml[128 + r], M = fmaxf(m, m1);
-        // a sum without a max is NaN, and stays
-        const float f0 = l == 0.f ? 0.f : m == -INFINITY ? 1.f : ex2(m - M);
-        const float f1 = l1 == 0.f ? 0.f : m1 == -INFINITY ? 1.f : ex2(m1 - M);
-#pragma unroll
-        for (int d = 0; d < VP / 2; ++d) {
-          const f32x2 c = f1 == 0.f ? pk(0.f, 0.f) : mul2(xch[d * 128 + r], pk(f1, f1));
-          o[d] = add2(f0 == 0.f ? pk(0.f, 0.f) : mul2(o[d], pk(f0, f0)), c);
-        }
-        l = (f0 == 0.f ? 0.f : f0 * l) + (f1 == 0.f ? 0.f : f1 * l1);
-        m = M;
-      }
-    }
-    if (wg == 0 && mine && !is_slow) {
+    if (mine && !is_slow) {
+      const int d0 = wg * 64;
       if (A.nsplit > 1) {
         float* dst = A.part + ((((size_t)b * A.kvh + kh) * A.nsplit + z) * R + rr) * (A.vh + 2);
 #pragma unroll
-        for (int d = 0; d < VP; d += 2)
-          if (d < A.vh) *reinterpret_cast<f32x2*>(dst + d) = o[d / 2];
-        *reinterpret_cast<float2*>(dst + A.vh) = make_float2(m, l);
+        for (int d = 0; d < 64; d += 2)
+          if (d0 + d < A.vh) *reinterpret_cast<f32x2*>(dst + d0 + d) = o[d / 2];
+        if (wg == 0) *reinterpret_cast<float2*>(dst + A.vh) = make_float2(m, l);
       } else {
         float* dst = A.out + (node_at * A.heads + head) * A.vh;
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int d = 0; d < VP; d += 4)  // vh and the start of out are multiples of four floats
-          if (d < A.vh)
-            *reinterpret_cast<ulonglong2*>(dst + d) =
+        for (int d = 0; d < 64; d += 4)  // vh and the start of out are multiples of four floats
+          if (d0 + d < A.vh)
+            *reinterpret_cast<ulonglong2*>(dst + d0 + d) =
                 make_ulonglong2(mul2(o[d / 2], pk(inv, inv)), mul2(o[d / 2 + 1], pk(inv, inv)));
       }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_PROD));
-    const int role = warp & 3, set = wg - W;  // 0 keys, 1 and 2 values of the steps of warpgroup `set`, 3 MMA
-    if (role == 3 && set > 0) {
-      // nothing to do
-    } else if (role == 3) {
+    const int role = warp & 3;  // 0 keys, 1 and 2 values, 3 MMA
+    if (role == 3) {
       // ---------------------------------------------------------- MMA issue
       const uint64_t dq_hi = sw128_desc(qhi), dq_lo = sw128_desc(qlo), d_stage = sw128_desc(stages);
       auto issue_qk = [&](int i) {  // S of step i
-        const int st = i % NST, w = i % W, jj = i / W;
+        const int st = i % NST;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t dk = d_stage + (uint64_t)(st * (C::STAGE >> 4));
-          const uint32_t d = tmem + w * C::WG_COLS + (jj & 1) * BN;
+          const uint32_t d = tmem + (i & 1) * BN;
           uint32_t acc = 0;
           auto steps = [&](uint64_t dq, uint64_t dkk) {
 #pragma unroll
@@ -658,52 +604,50 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           steps(dq_lo, dk);
           if (!I8) steps(dq_hi, dk + (uint64_t)(C::K_TILE >> 4));
           steps(dq_hi, dk);
-          umma_commit(&s_full[2 * w + (jj & 1)]);
+          umma_commit(&s_full[i & 1]);
         }
         __syncwarp();
       };
       auto issue_pv = [&](int i) {  // O of step i
-        const int st = i % NST, w = i % W, jj = i / W;
+        const int st = i % NST;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t dv = d_stage + (uint64_t)((st * C::STAGE + C::PARTS * C::K_TILE) >> 4);
-          const uint32_t at = tmem + w * C::WG_COLS, p = at + (jj & 1) * BN;
+          const uint32_t p = tmem + (i & 1) * BN;
           uint32_t acc = 0;
           auto steps = [&](uint32_t a, uint64_t dvv) {
 #pragma unroll
             for (int k = 0; k < BN / 16; ++k) {
-              mma_ts<VP>(at + 2 * BN, a + k * 16, dvv + (uint64_t)(k * 2), acc);
+              mma_ts<VP>(tmem + 2 * BN, a + k * 16, dvv + (uint64_t)(k * 2), acc);
               acc = 1;
             }
           };
           steps(p + 8, dv);
           if (!I8) steps(p, dv + (uint64_t)(C::V_TILE >> 4));
           steps(p, dv);
-          umma_commit(&o_full[w]);
+          umma_commit(o_full);
           umma_commit(&empty[st]);
         }
         __syncwarp();
       };
-      // The scores of the first two steps of a warpgroup, then after each second
-      // product scores again: they take the place of the weights of step q - 2 W,
-      // whose product must be done. With two warpgroups they follow one product
-      // later, so that the wait for it is over when it begins.
+      // The scores of the first two steps, then after each second product scores
+      // again: they take the place of that step's weights, so the product must be
+      // done.
       auto scores = [&](int q) {
         bool ready = mbar_wait_asleep(&full[q % NST], (uint32_t)(q / NST) & 1u, abort, werr);
-        if (ready && q >= 2 * W) ready = mbar_wait_asleep(&o_full[q % W], (uint32_t)(q / W) & 1u, abort, werr);
+        if (ready && q >= 2) ready = mbar_wait_asleep(o_full, (uint32_t)q & 1u, abort, werr);
         ready = __all_sync(0xffffffffu, ready);
         if (ready) issue_qk(q);
         return ready;
       };
       bool ok = nblk == 0 || mbar_wait_asleep(q_full, 0, abort, werr);
       ok = __all_sync(0xffffffffu, ok);
-      constexpr int AHEAD = 2 * W - (W - 1);  // steps from a second product to the scores issued after it
-      for (int q = 0; q < AHEAD && q < nblk && ok; ++q) ok = scores(q);
+      for (int q = 0; q < 2 && q < nblk && ok; ++q) ok = scores(q);
       for (int i = 0; i < nblk && ok; ++i) {
-        ok = mbar_wait_asleep(&p_full[i % W], (uint32_t)(i / W) & 1u, abort, werr);
+        ok = mbar_wait_asleep(p_full, (uint32_t)i & 1u, abort, werr);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) issue_pv(i);
-        if (ok && i + AHEAD < nblk) ok = scores(i + AHEAD);
+        if (ok && i + 2 < nblk) ok = scores(i + 2);
       }
       // Every issued MMA completes before TMEM is freed.
       if (elect_one()) umma_commit(drain);
@@ -714,9 +658,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       bool ok = true;
       int e = 14, low = 255;
       // int8: positions lane and lane + 32 of a step and their scales; the next
-      // step's are on their way while one is widened (of wide keys, whose second
-      // set of warps is at work meanwhile, none).
-      constexpr bool AHEAD = I8 && W == 1;
+      // step's are on their way while one is widened.
       uint4 kn[2][QS];
       float ksn[2], vsn[2];
       auto load = [&](int i) {
@@ -729,14 +671,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           ksn[h] = in ? __ldg((d ? A.tks : A.ks) + row) : 0.f;
           vsn[h] = in ? __ldg((d ? A.tvs : A.vs) + row) : 0.f;
           const uint4* src = reinterpret_cast<const uint4*>((d ? A.tk : A.k) + row * A.qk);
-          if (AHEAD || h == 0) {
 #pragma unroll
-            for (int c = 0; c < QS; ++c) kn[h][c] = in && c * 16 < A.qk ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-          }
+          for (int c = 0; c < QS; ++c) kn[h][c] = in && c * 16 < A.qk ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
         }
       };
-      if (I8 && set < nblk) load(set);
-      for (int i = set; i < nblk; i += W) {
+      if (I8 && nblk > 0) load(0);
+      for (int i = 0; i < nblk; ++i) {
         const int st = i % NST, v0 = (blk0 + i) * BN;
         unsigned char* kt = stages + (size_t)st * C::STAGE;
         float ksc[2], vsc[2];
@@ -750,16 +690,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
             ksc[h] = ksn[h], vsc[h] = vsn[h];
             uint4 kk[QS];
 #pragma unroll
-            for (int c = 0; c < QS; ++c) kk[c] = kn[AHEAD ? h : 0][c];
-            if (!AHEAD && h == 0) {
-              const int v = v0 + 32 + lane;
-              const bool in = v < P.total;
-              const uint4* src =
-                  reinterpret_cast<const uint4*>((P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk);
-#pragma unroll
-              for (int c = 0; c < QS; ++c) kn[0][c] = in && c * 16 < A.qk ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-            }
-            if (AHEAD && h == 1 && i + W < nblk) load(i + W);
+            for (int c = 0; c < QS; ++c) kk[c] = kn[h][c];
+            if (h == 1 && i + 1 < nblk) load(i + 1);
 #pragma unroll
             for (int c = 0; c < QS; ++c) {
               uint32_t w[8];
@@ -774,7 +706,6 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
             }
             sane[h] = fabsf(ksc[h]) <= 3.4028234e38f && fabsf(vsc[h]) <= 3.4028234e38f;
           }
-          if (!AHEAD && i + W < nblk) load(i + W);
           // Value scales, held so that the largest so far is in [2^13, 2^14).
           uint32_t top = 0, least = 0x7f800000u;
 #pragma unroll
@@ -848,7 +779,6 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       // lanes in different chunks. The next step's values are on their way while
       // one is widened.
       constexpr int DV = VP / 8;
-      constexpr bool AHEAD = I8 && W == 1;
       const int d0 = (vw * 4 + (lane >> 3)) * DV;
       uint32_t xn[8][DV / 4];
       auto get = [&](const char* src, bool in, uint32_t (&x)[DV / 4]) {
@@ -875,8 +805,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           }
         }
       };
-      if (I8 && set < nblk) load(set);
-      for (int i = set; i < nblk; i += W) {
+      if (I8 && nblk > 0) load(0);
+      for (int i = 0; i < nblk; ++i) {
         const int st = i % NST, v0 = (blk0 + i) * BN;
         unsigned char* vt = stages + (size_t)st * C::STAGE + C::PARTS * C::K_TILE;
         if (I8) {
@@ -886,7 +816,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int q = 0; q < DV / 4; ++q) x[j][q] = xn[j][q];
-          if (AHEAD && i + W < nblk) load(i + W);
+          if (i + 1 < nblk) load(i + 1);
           if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
           __syncwarp();
           if (d0 < A.vh) {
@@ -907,7 +837,6 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               }
             }
           }
-          if (!AHEAD && i + W < nblk) load(i + W);
         } else {
           // f32: a warp holds 32 positions (four octets) whole, four dims a lane
           // in each of two rounds, so a position's largest value is the warp's
@@ -1052,11 +981,11 @@ cudaError_t launch_umma_form(const TreeArgs& A, int B, cudaStream_t st) {
   return cudaSuccess;
 }
 
-typedef TreeUmma<true, 3, 64, 1, 4> UmmaI8x48;
-typedef TreeUmma<true, 4, 64, 1, 4> UmmaI8x64;
-typedef TreeUmma<true, 8, 128, 2, 4> UmmaI8x128;
-typedef TreeUmma<false, 3, 64, 1, 2> UmmaF32x48;
-typedef TreeUmma<false, 4, 64, 1, 2> UmmaF32x64;
+typedef TreeUmma<true, 3, 64, 4> UmmaI8x48;
+typedef TreeUmma<true, 4, 64, 4> UmmaI8x64;
+typedef TreeUmma<true, 8, 128, 4> UmmaI8x128;
+typedef TreeUmma<false, 3, 64, 2> UmmaF32x48;
+typedef TreeUmma<false, 4, 64, 2> UmmaF32x64;
 
 }  // namespace
 
