@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
   constexpr bool I8 = C::I8;
   constexpr int BN = C::BN, VP = C::VP, QS = C::QS, TPR = C::TPR, CW = C::CW, NST = C::NST, NC = BN / 32;
   extern __shared__ unsigned char raw[];
-  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  // An offset, not a rounded integer: the compiler keeps track of the address space.
+  unsigned char* sm = raw + ((0u - su32(raw)) & 1023u);
   unsigned char *qhi = sm, *qlo = sm + C::Q_TILE, *stages = sm + 2 * C::Q_TILE;
   float* col_k = reinterpret_cast<float*>(stages + (size_t)NST * C::STAGE);  // [NST][BN] key scales
   float* col_v = col_k + NST * BN;                                          // [NST][BN] value scales times 2^(140 - e)
@@ -408,8 +409,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
     int low = 255;
     for (int i = 0; i < nj; ++i) {
       const int st = i % NST;
-      if (ok && !mbar_wait_asleep(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, abort, werr)) ok = false;
-      if (ok && !mbar_wait_asleep(&full[st], (uint32_t)(i / NST) & 1u, abort, werr)) ok = false;
+      if (ok && !mbar_wait_spin(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, abort, werr)) ok = false;
+      if (ok && !mbar_wait_spin(&full[st], (uint32_t)(i / NST) & 1u, abort, werr)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       float mx = -INFINITY;
       f32x2 s[CW / 2];
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         // ---- weights: sum, and times the value scale as f16 parts into S's place
         // (16 positions' columns take 8 of high parts, then 8 of remainders)
         f32x2 add = pk(0.f, 0.f);
-        const f32x2 qs2 = pk(qs, qs), mz2 = pk(-mz, -mz);
+        const f32x2 qs2 = pk(qs, qs), mz2 = pk(-mz, -mz), minus = pk(-1.f, -1.f);
 #pragma unroll
         for (int c = 0; c < CW / 16; ++c) {
           uint32_t hi[8], lo[8];
@@ -479,11 +480,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               up(fma2(s[8 * c + 2 * j + g], qs2, mz2), f0, f1);
               const f32x2 p = pk(ex2(f0), ex2(f1));
               add = add2(add, p);
-              up(mul2(p, g ? pk(vv.z, vv.w) : pk(vv.x, vv.y)), w0, w1);
-              const float t0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u),
-                          t1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
-              hi[2 * j + g] = cvt2(t0, t1);
-              lo[2 * j + g] = cvt2(w0 - t0, w1 - t1);
+              const f32x2 w = mul2(p, g ? pk(vv.z, vv.w) : pk(vv.x, vv.y));
+              const f32x2 t = w & 0xffffe000ffffe000ull;
+              up(t, w0, w1);
+              hi[2 * j + g] = cvt2(w0, w1);
+              up(fma2(t, minus, w), w0, w1);
+              lo[2 * j + g] = cvt2(w0, w1);
             }
           }
           tmem_st8(s_now + c * 16, hi);
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         const int e = expo[2 * st];
         low = expo[2 * st + 1];
         if (i > 0) {
-          if (!mbar_wait_asleep(o_full, (uint32_t)(i - 1) & 1u, abort, werr)) ok = false;
+          if (!mbar_wait_spin(o_full, (uint32_t)(i - 1) & 1u, abort, werr)) ok = false;
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
 #pragma unroll
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
     if (nj > 0) {
       float top = 0.f;
       bool faint = false;
-      if (ok && !mbar_wait_asleep(o_full, (uint32_t)(nj - 1) & 1u, abort, werr)) ok = false;
+      if (ok && !mbar_wait_spin(o_full, (uint32_t)(nj - 1) & 1u, abort, werr)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
@@ -634,17 +636,17 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       // again: they take the place of that step's weights, so the product must be
       // done.
       auto scores = [&](int q) {
-        bool ready = mbar_wait_asleep(&full[q % NST], (uint32_t)(q / NST) & 1u, abort, werr);
-        if (ready && q >= 2) ready = mbar_wait_asleep(o_full, (uint32_t)q & 1u, abort, werr);
+        bool ready = mbar_wait_spin(&full[q % NST], (uint32_t)(q / NST) & 1u, abort, werr);
+        if (ready && q >= 2) ready = mbar_wait_spin(o_full, (uint32_t)q & 1u, abort, werr);
         ready = __all_sync(0xffffffffu, ready);
         if (ready) issue_qk(q);
         return ready;
       };
-      bool ok = nblk == 0 || mbar_wait_asleep(q_full, 0, abort, werr);
+      bool ok = nblk == 0 || mbar_wait_spin(q_full, 0, abort, werr);
       ok = __all_sync(0xffffffffu, ok);
       for (int q = 0; q < 2 && q < nblk && ok; ++q) ok = scores(q);
       for (int i = 0; i < nblk && ok; ++i) {
-        ok = mbar_wait_asleep(p_full, (uint32_t)i & 1u, abort, werr);
+        ok = mbar_wait_spin(p_full, (uint32_t)i & 1u, abort, werr);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) issue_pv(i);
         if (ok && i + 2 < nblk) ok = scores(i + 2);
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         float ksc[2], vsc[2];
         bool sane[2];
         if (I8) {
-          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
           __syncwarp();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -728,7 +730,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         } else {
           // f32: each key scaled by the power of two that brings its largest
           // element into [2^13, 2^14); the values' scales are the value warps' matter.
-          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
           __syncwarp();
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
@@ -817,7 +819,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
 #pragma unroll
             for (int q = 0; q < DV / 4; ++q) x[j][q] = xn[j][q];
           if (i + 1 < nblk) load(i + 1);
-          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
           __syncwarp();
           if (d0 < A.vh) {
 #pragma unroll
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           }
           top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
           bad = __reduce_or_sync(0xffffffffu, bad);
-          if (ok && !mbar_wait_asleep(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+          if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
           __syncwarp();
           if (lane == 0) vmax[(i & 1) * 4 + vw] = top, vmax[(i & 1) * 4 + 2 + vw] = least;
           asm volatile("bar.sync 4, 64;" ::: "memory");

@@ -36,20 +36,6 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// As mbar_try, but asleep until the phase completes or about a millisecond has
-// gone by: a waiting warp then issues nothing.
-__device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(su32(bar)), "r"(parity), "r"(1000000u)
-      : "memory");
-  return ok != 0;
-}
-
 // Wait for phase `parity` of `bar`. Gives up after WAIT_NS (raising *werr) or
 // as soon as another role of the CTA gave up (`abort`), returning false. Between polls a
 // waiter sleeps `backoff_ns` so waiting warps leave the issue slots to the
@@ -70,14 +56,17 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-// mbar_wait asleep, bounded by the SM's clock (about a second), whose reading
-// costs a few cycles where the global timer's costs hundreds.
+// mbar_wait for short waits between warps of a block: a bare loop on the
+// barrier, which the hardware holds for a while per try (a time hint would put a
+// software sleep between two tries), bounded by the SM's clock (about a second),
+// whose reading costs a few cycles where the global timer's costs hundreds.
 constexpr long long WAIT_CLOCKS = 1ll << 31;
-__device__ __forceinline__ bool mbar_wait_asleep(uint64_t* bar, uint32_t parity, volatile uint32_t* abort, int* werr) {
-  if (mbar_sleep(bar, parity)) return true;
+__device__ __forceinline__ bool mbar_wait_spin(uint64_t* bar, uint32_t parity, volatile uint32_t* abort, int* werr) {
   const long long t0 = clock64();
   while (true) {
-    if (mbar_sleep(bar, parity)) return true;
+#pragma unroll 1
+    for (int n = 0; n < 64; ++n)
+      if (mbar_try(bar, parity)) return true;
     if (*abort) return false;
     if (clock64() - t0 > WAIT_CLOCKS) {
       *abort = 1;
