@@ -1,5 +1,5 @@
-// nd_attend_tree on the 5th-generation tensor cores, for trees whose T * rep
-// rows of a KV head fill most of a 128-row MMA tile (tree_kernels.cu says when).
+// nd_attend_tree on the 5th-generation tensor cores, for trees with more than 16
+// rows (T * rep) of a KV head.
 //
 //   S = Q K^T,  P = 2^(S * scales - max),  O += P V
 //
@@ -729,43 +729,54 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           if (lane == 0) expo[2 * st] = e, expo[2 * st + 1] = low;
         } else {
           // f32: each key scaled by the power of two that brings its largest
-          // element into [2^13, 2^14); the values' scales are the value warps' matter.
+          // element into [2^13, 2^14); the values' scales are the value warps'
+          // matter. A key over 64 wide is two lanes', 64 elements each.
+          constexpr int KP = 32 / C::KA, KX = C::KA == 1 ? QS * 4 : 16;
+          const int part = lane / KP;
+          uint32_t outs = 0;
           if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
           __syncwarp();
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            const int kp = h * 32 + lane, v = v0 + kp;
+          for (int h = 0; h < BN / KP; ++h) {
+            const int kp = h * KP + lane % KP, v = v0 + kp, d0 = part * 64;
             const bool in = v < P.total;
             const float4* src = reinterpret_cast<const float4*>(
                 reinterpret_cast<const float*>(P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk);
-            float4 x[QS * 4];
+            float4 x[KX];
 #pragma unroll
-            for (int c = 0; c < QS * 4; ++c) x[c] = in && c * 4 < A.qk ? __ldg(src + c) : make_float4(0, 0, 0, 0);
+            for (int c = 0; c < KX; ++c)
+              x[c] = in && d0 + c * 4 < A.qk ? __ldg(src + part * 16 + c) : make_float4(0, 0, 0, 0);
             float mx = 0.f;
             bool fine = true;
 #pragma unroll
-            for (int c = 0; c < QS * 4; ++c) {
+            for (int c = 0; c < KX; ++c) {
               const float a = fmaxf(fmaxf(fabsf(x[c].x), fabsf(x[c].y)), fmaxf(fabsf(x[c].z), fabsf(x[c].w)));
               const float t = fabsf(x[c].x) + fabsf(x[c].y) + fabsf(x[c].z) + fabsf(x[c].w);  // NaN where one is
               fine &= a <= 3.4028234e38f && t == t;
               mx = fmaxf(mx, a);
             }
+            if (C::KA == 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             const int ef = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
             const float by = __uint_as_float((uint32_t)(267 - ef) << 23);
 #pragma unroll
-            for (int c = 0; c < QS * 2; ++c) {
+            for (int c = 0; c < KX / 2; ++c) {
               uint32_t hh[4], ll[4];
               halves(x[2 * c].x * by, x[2 * c].y * by, &hh[0], &ll[0]);
               halves(x[2 * c].z * by, x[2 * c].w * by, &hh[1], &ll[1]);
               halves(x[2 * c + 1].x * by, x[2 * c + 1].y * by, &hh[2], &ll[2]);
               halves(x[2 * c + 1].z * by, x[2 * c + 1].w * by, &hh[3], &ll[3]);
-              unsigned char* at = kt + kp * 128 + ((c ^ (kp & 7)) << 4);
+              unsigned char* at = kt + part * (BN * 128) + kp * 128 + ((c ^ (kp & 7)) << 4);
               *reinterpret_cast<uint4*>(at) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
               *reinterpret_cast<uint4*>(at + C::K_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
             }
-            col_k[st * BN + kp] = in ? __uint_as_float((uint32_t)(ef - 13) << 23) : 0.f;
-            const uint32_t w = __ballot_sync(0xffffffffu, !fine);
-            if (lane == 0) odd[st * 2 * NC + h] = w;
+            if (part == 0) col_k[st * BN + kp] = in ? __uint_as_float((uint32_t)(ef - 13) << 23) : 0.f;
+            uint32_t w = __ballot_sync(0xffffffffu, !fine);
+            if (C::KA == 2) w = (w | w >> 16) & 0xffffu;
+            outs |= w << (h * KP & 31);
+            if (((h + 1) * KP & 31) == 0) {
+              if (lane == 0) odd[st * 2 * NC + (h * KP >> 5)] = outs;
+              outs = 0;
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -840,85 +851,95 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
             }
           }
         } else {
-          // f32: a warp holds 32 positions (four octets) whole, four dims a lane
-          // in each of two rounds, so a position's largest value is the warp's
-          // own matter. A value is scaled like a key; 2^(140 - e) is a step's
-          // share of the scale, by the largest exponent of both warps so far.
-          const int oc = lane & 3, pr = vw * 4 + oc;
-          auto row_of = [&](int j) {  // position j of the octet, null past the end
-            const int vj = v0 + pr * 8 + j;
-            return vj < P.total ? reinterpret_cast<const float*>(P.in_draft(vj) ? A.tv : A.v) + P.row(vj) * A.vh : nullptr;
-          };
+          // f32: a warp holds 32 positions (four octets; of 128-wide values two
+          // at a time) whole, four dims a lane in each of two rounds, so a
+          // position's largest value is the warp's own matter. A value is scaled
+          // like a key; 2^(140 - e) is a step's share of the scale, by the largest
+          // exponent of both warps so far.
+          constexpr int OCT = VP == 64 ? 4 : 2, PASS = 4 / OCT, DR = 128 / OCT;
+          const int oc = lane % OCT;
           auto at = [&](const float* row, int d) {
             return row && d < A.vh ? __ldg(reinterpret_cast<const float4*>(row + d)) : make_float4(0, 0, 0, 0);
           };
-          float4 x[2][8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float* row = row_of(j);
-            x[0][j] = at(row, (lane >> 2) * 4), x[1][j] = at(row, 32 + (lane >> 2) * 4);
-          }
           // Exponent field of each position's largest value (0 none, 255 not finite), a byte a position.
           int top = 0, least = 255;
-          uint32_t ef[2] = {0, 0}, bad = 0;
+          uint32_t ef[PASS][2], bad = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 f = x[0][j], g = x[1][j];
-            float a = fmaxf(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))),
-                            fmaxf(fmaxf(fabsf(g.x), fabsf(g.y)), fmaxf(fabsf(g.z), fabsf(g.w))));
-            const float t = fabsf(f.x) + fabsf(f.y) + fabsf(f.z) + fabsf(f.w) + fabsf(g.x) + fabsf(g.y) + fabsf(g.z) +
-                            fabsf(g.w);  // NaN where one is
-            if (t != t) a = INFINITY;
+          for (int p = 0; p < PASS; ++p) {
+            const int pr = vw * 4 + p * OCT + oc, da = lane / OCT * 4;
+            float4 x[2][8];
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-            const int y = a == 0.f ? 0 : a <= 3.4028234e38f ? min(max((int)(__float_as_uint(a) >> 23), 14), 253) : 255;
-            if (y == 255) bad |= 1u << (8 * oc + j);
-            else if (y > 0) top = max(top, y - 13), least = min(least, y - 13);
-            ef[j >> 2] |= (uint32_t)y << (8 * (j & 3));
+            for (int j = 0; j < 8; ++j) {
+              const int vj = v0 + pr * 8 + j;
+              const float* row =
+                  vj < P.total ? reinterpret_cast<const float*>(P.in_draft(vj) ? A.tv : A.v) + P.row(vj) * A.vh : nullptr;
+              x[0][j] = at(row, da), x[1][j] = at(row, DR + da);
+            }
+            ef[p][0] = ef[p][1] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = x[0][j], g = x[1][j];
+              float a = fmaxf(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))),
+                              fmaxf(fmaxf(fabsf(g.x), fabsf(g.y)), fmaxf(fabsf(g.z), fabsf(g.w))));
+              const float t = fabsf(f.x) + fabsf(f.y) + fabsf(f.z) + fabsf(f.w) + fabsf(g.x) + fabsf(g.y) + fabsf(g.z) +
+                              fabsf(g.w);  // NaN where one is
+              if (t != t) a = INFINITY;
+#pragma unroll
+              for (int d = OCT; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+              const int y = a == 0.f ? 0 : a <= 3.4028234e38f ? min(max((int)(__float_as_uint(a) >> 23), 14), 253) : 255;
+              if (y == 255) bad |= 1u << (8 * (p * OCT + oc) + j);
+              else if (y > 0) top = max(top, y - 13), least = min(least, y - 13);
+              ef[p][j >> 2] |= (uint32_t)y << (8 * (j & 3));
+            }
+            if (p == 0) {
+              if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+              __syncwarp();
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int d0 = h * DR + da;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int y = (int)((ef[p][j >> 2] >> (8 * (j & 3))) & 255u);
+                const bool use = y > 0 && y < 255;  // nothing of one that is not finite
+                const float by = __uint_as_float((uint32_t)(267 - (use ? y : 140)) << 23);
+                x[h][j].x = use ? x[h][j].x * by : 0.f, x[h][j].y = use ? x[h][j].y * by : 0.f;
+                x[h][j].z = use ? x[h][j].z * by : 0.f, x[h][j].w = use ? x[h][j].w * by : 0.f;
+              }
+              if (d0 >= A.vh) continue;
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                uint32_t hh[4], ll[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float4 a = x[h][2 * j], c = x[h][2 * j + 1];
+                  halves(t == 0 ? a.x : t == 1 ? a.y : t == 2 ? a.z : a.w, t == 0 ? c.x : t == 1 ? c.y : t == 2 ? c.z : c.w,
+                         &hh[j], &ll[j]);
+                }
+                const int d = d0 + t;
+                unsigned char* to = vt + d * 128 + ((pr ^ (d & 7)) << 4);
+                *reinterpret_cast<uint4*>(to) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
+                *reinterpret_cast<uint4*>(to + C::V_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
+              }
+            }
           }
           top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
           bad = __reduce_or_sync(0xffffffffu, bad);
-          if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
-          __syncwarp();
           if (lane == 0) vmax[(i & 1) * 4 + vw] = top, vmax[(i & 1) * 4 + 2 + vw] = least;
           asm volatile("bar.sync 4, 64;" ::: "memory");
           e = max(e, max(vmax[(i & 1) * 4], vmax[(i & 1) * 4 + 1]));
           low = min(low, min(vmax[(i & 1) * 4 + 2], vmax[(i & 1) * 4 + 3]));
           if (lane == 0) odd[st * 2 * NC + NC + vw] = bad;
           if (vw == 0 && lane == 0) expo[2 * st] = e, expo[2 * st + 1] = low;
-          if (lane < 4) {
+          if (lane < OCT) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int x = (int)((ef[j >> 2] >> (8 * (j & 3))) & 255u), f = 127 + x - e;  // 2^(x - 140) 2^(140 - e)
-              col_v[st * BN + pr * 8 + j] = x > 0 && x < 255 && f > 0 ? __uint_as_float((uint32_t)f << 23) : 0.f;
-            }
-          }
+            for (int p = 0; p < PASS; ++p)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int d0 = h * 32 + (lane >> 2) * 4;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int y = (int)((ef[j >> 2] >> (8 * (j & 3))) & 255u);
-              const bool use = y > 0 && y < 255;  // nothing of one that is not finite
-              const float by = __uint_as_float((uint32_t)(267 - (use ? y : 140)) << 23);
-              x[h][j].x = use ? x[h][j].x * by : 0.f, x[h][j].y = use ? x[h][j].y * by : 0.f;
-              x[h][j].z = use ? x[h][j].z * by : 0.f, x[h][j].w = use ? x[h][j].w * by : 0.f;
-            }
-            if (d0 >= A.vh) continue;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              uint32_t hh[4], ll[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float4 a = x[h][2 * j], c = x[h][2 * j + 1];
-                halves(t == 0 ? a.x : t == 1 ? a.y : t == 2 ? a.z : a.w, t == 0 ? c.x : t == 1 ? c.y : t == 2 ? c.z : c.w,
-                       &hh[j], &ll[j]);
+              for (int j = 0; j < 8; ++j) {
+                const int x = (int)((ef[p][j >> 2] >> (8 * (j & 3))) & 255u), f = 127 + x - e;  // 2^(x - 140) 2^(140 - e)
+                col_v[st * BN + (vw * 4 + p * OCT + oc) * 8 + j] =
+                    x > 0 && x < 255 && f > 0 ? __uint_as_float((uint32_t)f << 23) : 0.f;
               }
-              const int d = d0 + t;
-              unsigned char* to = vt + d * 128 + ((pr ^ (d & 7)) << 4);
-              *reinterpret_cast<uint4*>(to) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
-              *reinterpret_cast<uint4*>(to + C::V_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
-            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -988,12 +1009,21 @@ typedef TreeUmma<true, 4, 64, 4> UmmaI8x64;
 typedef TreeUmma<true, 8, 128, 4> UmmaI8x128;
 typedef TreeUmma<false, 3, 64, 2> UmmaF32x48;
 typedef TreeUmma<false, 4, 64, 2> UmmaF32x64;
+typedef TreeUmma<false, 8, 128, 2> UmmaF32x128;
 
 }  // namespace
 
+// More than 16 rows, whole 16-byte pieces and MMA steps. A step costs nearly the
+// same for 17 rows as for 128; mma.sync pays per 16 rows. Measured, mma.sync -> here:
+//   rows   48/64 int8, 256 x 1043   48/64 f32, 128 x 1043   128 int8, 4 x 16000   128 f32, 2 x 8000
+//    12        71 ->  63 us              68 ->  83 us            100 -> 111 us
+//    16                                                                              134 us -> (not taken)
+//    24       129 ->  64                114 ->  83               157 -> 112          220 -> 135
+//    48       127 ->  74                202 ->  85               251 -> 116          304 -> 136 (36 rows)
+//    96       192 ->  79                211 ->  90               383 -> 125          750 -> 150 (128 rows)
+// and at eight sessions of 1043 (48/64 int8) 12 rows 15 -> 19, 24 rows 21 -> 19.
 bool tree_umma_takes(int int8, int rows, int qk, int vh, int piece) {
-  if (piece != 16 || qk % 16 || vh % 16 || rows < 48) return false;
-  return int8 || (qk <= 64 && vh <= 64);
+  return piece == 16 && qk % 16 == 0 && vh % 16 == 0 && rows > 16;
 }
 
 // Splits that need the fewest rounds of blocks: a block of positions costs
@@ -1017,6 +1047,7 @@ cudaError_t launch_tree_umma(const TreeArgs& A, int int8, int B, cudaStream_t st
     if (A.qk > 48) return launch_umma_form<UmmaI8x64>(A, B, st);
     return launch_umma_form<UmmaI8x48>(A, B, st);
   }
+  if (A.qk > 64 || A.vh > 64) return launch_umma_form<UmmaF32x128>(A, B, st);
   if (A.qk > 48) return launch_umma_form<UmmaF32x64>(A, B, st);
   return launch_umma_form<UmmaF32x48>(A, B, st);
 }
