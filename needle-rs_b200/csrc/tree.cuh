@@ -52,7 +52,7 @@ inline TreeArgs tree_sessions(const TreeArgs& A, int b0, int es) {
 
 // Whether the tcgen05 form takes heads of these widths, and its launch.
 bool tree_umma_takes(int int8, int rows, int qk, int vh, int piece);
-int tree_umma_nsplit(int B, int rows, int kvh, int qk, int vh, int span);
+int tree_umma_nsplit(int int8, int B, int rows, int kvh, int qk, int vh, int span);
 cudaError_t launch_tree_umma(const TreeArgs& A, int int8, int B, cudaStream_t st);
 
 }  // namespace nb

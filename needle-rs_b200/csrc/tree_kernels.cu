@@ -773,7 +773,7 @@ TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv,
   P.piece = qk * es % 16 == 0 && vh * es % 16 == 0 && al16(k) && al16(v) && al16(tk) && al16(tv) ? 16 : 4;
   P.umma = al16(out) && tree_umma_takes(int8, R, qk, vh, P.piece);
   if (P.umma) {
-    P.nsplit = tree_umma_nsplit(B, R, kvh, qk, vh, slots + (tk ? T : 0));
+    P.nsplit = tree_umma_nsplit(int8, B, R, kvh, qk, vh, slots + (tk ? T : 0));
     P.part = P.nsplit > 1;
     return P;
   }

@@ -14,17 +14,19 @@
 // is drained into f32 registers after every block.
 //
 // Warps: one softmax warpgroup with a thread a row, or, for 128-wide heads,
-// whose outputs would fill a thread's registers, two with half of a row's
-// positions and half of its outputs each (they tell each other their maxima),
-// and one warpgroup of
-//   a key warp and two value warps, which read the ring and the draft, widen
-//   them to f16 and lay them down in the 128-byte swizzled form the MMA reads
-//   (keys as they lie, values transposed eight positions at a time in
-//   registers; the key warp also forms the steps' scales), and
+// whose outputs would fill a thread's registers, and for f32, two with half of a
+// row's positions and half of its outputs each (they tell each other their
+// maxima), and one warpgroup (f32: two) of
+//   a key warp and two value warps (f32: two and four, whose conversion is what
+//   bounds a step: a chain of 3300 cycles of 64 positions, 5400 with the maxima
+//   of eight positions reduced one after another), which read the ring and the
+//   draft, turn them to f16 and lay them down in the 128-byte swizzled form the
+//   MMA reads (keys as they lie, values transposed eight positions at a time in
+//   registers; of int8 the key warp also forms the steps' scales), and
 //   an MMA warp, which issues every product as soon as its operands stand: a
 //   warp that issues MMAs is held for as long as they run.
-// Heads of up to 64 leave room for two blocks on an SM, which hide each other's
-// latencies; 128-wide heads need the shared memory of a whole SM.
+// int8 heads of up to 64 leave room for two blocks on an SM, which hide each
+// other's latencies; the others take a whole SM.
 //
 // Every wait is bounded as in umma_gemm.cu.
 #include <algorithm>
@@ -37,12 +39,13 @@
 namespace nb {
 namespace {
 
-template <bool I8_, int QS_, int VP_, int NST_>
+template <bool I8_, int QS_, int VP_, int TPR_, int NST_>
 struct TreeUmma {
   static constexpr bool I8 = I8_;
   static constexpr int QS = QS_;        // k16 steps of the key product
   static constexpr int VP = VP_;        // value width held (64 or 128)
-  static constexpr int TPR = VP / 64;   // softmax threads a row
+  static constexpr int TPR = TPR_;      // softmax threads a row
+  static constexpr int OW = VP / TPR;   // outputs of a softmax thread
   static constexpr int NST = NST_;
   static constexpr int BN = 64;         // positions of a stage, and of a step of the softmax
   static constexpr int CW = BN / TPR;   // positions of a softmax thread's step
@@ -50,12 +53,17 @@ struct TreeUmma {
   static constexpr int PARTS = I8 ? 1 : 2;        // high part, remainder
   static constexpr int Q_TILE = KA * 128 * 128, K_TILE = KA * BN * 128, V_TILE = VP * 128;
   static constexpr int STAGE = PARTS * (K_TILE + V_TILE);
-  static constexpr int THREADS = (TPR + 1) * 128, CTAS = TPR == 1 ? 2 : 1;
-  // Registers a thread: the launch's, a softmax thread's, the other warpgroup's;
+  static constexpr int PWG = I8 ? 1 : 2;        // warpgroups that read keys and values and issue MMAs
+  static constexpr int KW = I8 ? 1 : 2, VW = I8 ? 2 : 4;  // key and value warps among them
+  static constexpr int THREADS = (TPR + PWG) * 128, CTAS = I8 && TPR == 1 ? 2 : 1;
+  // Registers a thread: the launch's, a softmax thread's, the other warpgroups';
   // the warpgroups' shares add up to the launch's.
-  static constexpr int REG_ALL = TPR == 1 ? 128 : 168, REG_SOFT = TPR == 1 ? (I8 ? 184 : 160) : 176,
-                       REG_PROD = (TPR + 1) * REG_ALL - TPR * REG_SOFT;
-  static_assert(TPR * REG_SOFT + REG_PROD == (TPR + 1) * REG_ALL && REG_PROD % 8 == 0, "register shares");
+  static constexpr int REG_ALL = I8 && TPR == 2 ? 168 : 128,
+                       REG_SOFT = I8 ? (TPR == 1 ? 184 : 176) : VP == 64 ? 144 : 160,
+                       REG_PROD = ((TPR + PWG) * REG_ALL - TPR * REG_SOFT) / PWG;
+  static_assert(TPR * REG_SOFT + PWG * REG_PROD == (TPR + PWG) * REG_ALL && REG_PROD % 8 == 0 &&
+                    THREADS * CTAS * REG_ALL <= 65536,
+                "register shares");
   static constexpr int TMEM = 2 * BN + VP <= 128 ? 128 : 256;  // columns: two of S (then P), O
   static constexpr size_t META = NST * (size_t)(BN * 8 + 16 + 16) + 128 * 4 + 512 + 2 * 2 * 128 * 4;
   static constexpr size_t SMEM = 1024 + 2 * (size_t)Q_TILE + NST * (size_t)STAGE + META;
@@ -242,7 +250,7 @@ __device__ __noinline__ void tree_slow_row(const TreeArgs& A, const TreePlace& P
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __grid_constant__ TreeArgs A, int* werr) {
   constexpr bool I8 = C::I8;
-  constexpr int BN = C::BN, VP = C::VP, QS = C::QS, TPR = C::TPR, CW = C::CW, NST = C::NST, NC = BN / 32;
+  constexpr int BN = C::BN, VP = C::VP, QS = C::QS, TPR = C::TPR, OW = C::OW, CW = C::CW, NST = C::NST, NC = BN / 32;
   extern __shared__ unsigned char raw[];
   // An offset, not a rounded integer: the compiler keeps track of the address space.
   unsigned char* sm = raw + ((0u - su32(raw)) & 1023u);
@@ -263,7 +271,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
   volatile uint32_t* abort = tmem_slot + 1;
   int* range = reinterpret_cast<int*>(tmem_slot + 2);    // [2]
   uint32_t* slow = reinterpret_cast<uint32_t*>(range + 2);  // [4] rows for tree_slow_row
-  int* vmax = reinterpret_cast<int*>(slow + 4);             // [2][4] the value warps' exponents
+  int* vmax = reinterpret_cast<int*>(slow + 4);             // [2][8] the value warps' exponents
   float* both = reinterpret_cast<float*>(full) + 128;       // [2][2][128] what two threads of a row tell each other
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -277,7 +285,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
 
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
-      mbar_init(&full[s], 96);   // the key and value warps
+      mbar_init(&full[s], 32 * (C::KW + C::VW));  // the key and value warps
       mbar_init(&empty[s], 1);   // one tcgen05.commit
     }
     mbar_init(&s_full[0], 1);
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
     // ------------------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFT));
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + wg * CW, o_at = tmem + 2 * BN + wg * 64;  // the thread's columns of S and O
+    const uint32_t s_at = tmem + wg * CW, o_at = tmem + 2 * BN + wg * OW;  // the thread's columns of S and O
     // ---- queries: a row a thread of the first warpgroup, scaled by the power
     // of two that brings the row's max into [2^13, 2^14)
     if (wg == 0) {
@@ -387,11 +395,11 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       full0 = max(full0, __shfl_xor_sync(0xffffffffu, full0, d));
       full1 = min(full1, __shfl_xor_sync(0xffffffffu, full1, d));
     }
-    f32x2 o[32];  // dims 2 d, 2 d + 1 of the thread's 64
+    f32x2 o[OW / 2];  // dims 2 d, 2 d + 1 of the thread's
     float m = -INFINITY, l = 0.f;
     bool is_slow = false, ok = true;
 #pragma unroll
-    for (int d = 0; d < 32; ++d) o[d] = pk(0.f, 0.f);
+    for (int d = 0; d < OW / 2; ++d) o[d] = pk(0.f, 0.f);
     // Warps whose rows are all padding take no part.
     const int nj = (warp & 3) * 32 < rows ? nblk : 0;
     // What a thread has for the other of its row, and has from it; `turn`
@@ -502,7 +510,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           ok = __all_sync(0xffffffffu, ok);
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < 64; c += 32) {
+          for (int c = 0; c < OW; c += 32) {
             uint32_t x[2][16];
             tmem_ld16(o_at + lanes + c, x[0]);
             tmem_ld16(o_at + lanes + c + 16, x[1]);
@@ -514,7 +522,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           const float by = corr * (e - e_old > 126 ? 0.f : __uint_as_float((uint32_t)(127 - (e - e_old)) << 23));
           if (__any_sync(0xffffffffu, by != 1.f)) {
 #pragma unroll
-            for (int d2 = 0; d2 < 32; ++d2) o[d2] = mul2(o[d2], pk(by, by));
+            for (int d2 = 0; d2 < OW / 2; ++d2) o[d2] = mul2(o[d2], pk(by, by));
           }
         }
         e_old = e;
@@ -537,7 +545,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         const float by = __uint_as_float((uint32_t)(e_old - 13) << 23);
         bool bad = false;
 #pragma unroll
-        for (int c = 0; c < 64; c += 16) {
+        for (int c = 0; c < OW; c += 16) {
           uint32_t x[16];
           tmem_ld16(o_at + lanes + c, x);
           tmem_landed();
@@ -555,7 +563,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         faint = e_old - low > 12;
       } else {  // a wait gave up: the flag is up, and the rows say so
 #pragma unroll
-        for (int d = 0; d < 32; ++d) o[d] = pk(__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u));
+        for (int d = 0; d < OW / 2; ++d) o[d] = pk(__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u));
         l = 1.f, m = 0.f;
         is_slow = false;
       }
@@ -565,18 +573,18 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       if (TPR == 2) is_slow |= meet(~nj & 1, is_slow ? 1.f : 0.f) != 0.f;
     }
     if (mine && !is_slow) {
-      const int d0 = wg * 64;
+      const int d0 = wg * OW;
       if (A.nsplit > 1) {
         float* dst = A.part + ((((size_t)b * A.kvh + kh) * A.nsplit + z) * R + rr) * (A.vh + 2);
 #pragma unroll
-        for (int d = 0; d < 64; d += 2)
+        for (int d = 0; d < OW; d += 2)
           if (d0 + d < A.vh) *reinterpret_cast<f32x2*>(dst + d0 + d) = o[d / 2];
         if (wg == 0) *reinterpret_cast<float2*>(dst + A.vh) = make_float2(m, l);
       } else {
         float* dst = A.out + (node_at * A.heads + head) * A.vh;
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-        for (int d = 0; d < 64; d += 4)  // vh and the start of out are multiples of four floats
+        for (int d = 0; d < OW; d += 4)  // vh and the start of out are multiples of four floats
           if (d0 + d < A.vh)
             *reinterpret_cast<ulonglong2*>(dst + d0 + d) =
                 make_ulonglong2(mul2(o[d / 2], pk(inv, inv)), mul2(o[d / 2 + 1], pk(inv, inv)));
@@ -584,8 +592,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_PROD));
-    const int role = warp & 3;  // 0 keys, 1 and 2 values, 3 MMA
-    if (role == 3) {
+    const int pw = warp - TPR * 4;
+    if (pw == 3) {
       // ---------------------------------------------------------- MMA issue
       const uint64_t dq_hi = sw128_desc(qhi), dq_lo = sw128_desc(qlo), d_stage = sw128_desc(stages);
       auto issue_qk = [&](int i) {  // S of step i
@@ -655,7 +663,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       if (elect_one()) umma_commit(drain);
       __syncwarp();
       mbar_drain(drain, 0);
-    } else if (role == 0) {
+    } else if (pw == 0 || (!I8 && pw == 5)) {
       // ---------------------------------------------------------- keys and scales
       bool ok = true;
       int e = 14, low = 255;
@@ -677,7 +685,23 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           for (int c = 0; c < QS; ++c) kn[h][c] = in && c * 16 < A.qk ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
         }
       };
-      if (I8 && nblk > 0) load(0);
+      // f32: LK lanes a key, 32 / LK keys at a time.
+      constexpr int LK = 2 * C::KA, DL = QS * 16 / LK;
+      const int kw = pw == 0 ? 0 : 1;
+      float4 fn[DL / 4];
+      auto fetch = [&](int i, int u) {
+        const int v = (blk0 + i) * BN + kw * 32 + u * (32 / LK) + lane / LK, d0 = lane % LK * DL;
+        const bool in = v < P.total;
+        const float4* src = reinterpret_cast<const float4*>(
+            reinterpret_cast<const float*>(P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk);
+#pragma unroll
+        for (int c = 0; c < DL / 4; ++c)
+          fn[c] = in && d0 + c * 4 < A.qk ? __ldg(src + d0 / 4 + c) : make_float4(0, 0, 0, 0);
+      };
+      if (nblk > 0) {
+        if (I8) load(0);
+        else fetch(0, 0);
+      }
       for (int i = 0; i < nblk; ++i) {
         const int st = i % NST, v0 = (blk0 + i) * BN;
         unsigned char* kt = stages + (size_t)st * C::STAGE;
@@ -730,61 +754,56 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
         } else {
           // f32: each key scaled by the power of two that brings its largest
           // element into [2^13, 2^14); the values' scales are the value warps'
-          // matter. A key over 64 wide is two lanes', 64 elements each.
-          constexpr int KP = 32 / C::KA, KX = C::KA == 1 ? QS * 4 : 16;
-          const int part = lane / KP;
+          // matter. A warp has 32 positions, DL elements a lane; the next keys are
+          // on their way while some are converted.
           uint32_t outs = 0;
-          if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
-          __syncwarp();
-#pragma unroll 1
-          for (int h = 0; h < BN / KP; ++h) {
-            const int kp = h * KP + lane % KP, v = v0 + kp, d0 = part * 64;
-            const bool in = v < P.total;
-            const float4* src = reinterpret_cast<const float4*>(
-                reinterpret_cast<const float*>(P.in_draft(v) ? A.tk : A.k) + (in ? P.row(v) : 0) * A.qk);
-            float4 x[KX];
 #pragma unroll
-            for (int c = 0; c < KX; ++c)
-              x[c] = in && d0 + c * 4 < A.qk ? __ldg(src + part * 16 + c) : make_float4(0, 0, 0, 0);
-            float mx = 0.f;
-            bool fine = true;
+          for (int u = 0; u < LK; ++u) {
+            const int kp = kw * 32 + u * (32 / LK) + lane / LK;
+            float4 x[DL / 4];
 #pragma unroll
-            for (int c = 0; c < KX; ++c) {
-              const float a = fmaxf(fmaxf(fabsf(x[c].x), fabsf(x[c].y)), fmaxf(fabsf(x[c].z), fabsf(x[c].w)));
-              const float t = fabsf(x[c].x) + fabsf(x[c].y) + fabsf(x[c].z) + fabsf(x[c].w);  // NaN where one is
-              fine &= a <= 3.4028234e38f && t == t;
-              mx = fmaxf(mx, a);
+            for (int c = 0; c < DL / 4; ++c) x[c] = fn[c];
+            if (u + 1 < LK) fetch(i, u + 1);
+            else if (i + 1 < nblk) fetch(i + 1, 0);
+            float mx = 0.f, t = 0.f;  // t: NaN where one is
+#pragma unroll
+            for (int c = 0; c < DL / 4; ++c) {
+              mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[c].x), fabsf(x[c].y)), fmaxf(fabsf(x[c].z), fabsf(x[c].w))));
+              t += fabsf(x[c].x) + fabsf(x[c].y) + fabsf(x[c].z) + fabsf(x[c].w);
             }
-            if (C::KA == 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            if (t != t) mx = INFINITY;
+#pragma unroll
+            for (int d = 1; d < LK; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             const int ef = min(max((int)(__float_as_uint(mx) >> 23), 14), 253);
             const float by = __uint_as_float((uint32_t)(267 - ef) << 23);
+            if (u == 0) {
+              if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
+              __syncwarp();
+            }
 #pragma unroll
-            for (int c = 0; c < KX / 2; ++c) {
+            for (int c = 0; c < DL / 8; ++c) {
               uint32_t hh[4], ll[4];
               halves(x[2 * c].x * by, x[2 * c].y * by, &hh[0], &ll[0]);
               halves(x[2 * c].z * by, x[2 * c].w * by, &hh[1], &ll[1]);
               halves(x[2 * c + 1].x * by, x[2 * c + 1].y * by, &hh[2], &ll[2]);
               halves(x[2 * c + 1].z * by, x[2 * c + 1].w * by, &hh[3], &ll[3]);
-              unsigned char* at = kt + part * (BN * 128) + kp * 128 + ((c ^ (kp & 7)) << 4);
+              const int ch = lane % LK * (DL / 8) + c;
+              unsigned char* at = kt + (ch >> 3) * (BN * 128) + kp * 128 + (((ch & 7) ^ (kp & 7)) << 4);
               *reinterpret_cast<uint4*>(at) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
               *reinterpret_cast<uint4*>(at + C::K_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
             }
-            if (part == 0) col_k[st * BN + kp] = in ? __uint_as_float((uint32_t)(ef - 13) << 23) : 0.f;
-            uint32_t w = __ballot_sync(0xffffffffu, !fine);
-            if (C::KA == 2) w = (w | w >> 16) & 0xffffu;
-            outs |= w << (h * KP & 31);
-            if (((h + 1) * KP & 31) == 0) {
-              if (lane == 0) odd[st * 2 * NC + (h * KP >> 5)] = outs;
-              outs = 0;
-            }
+            if (lane % LK == 0) col_k[st * BN + kp] = v0 + kp < P.total ? __uint_as_float((uint32_t)(ef - 13) << 23) : 0.f;
+            if (!(mx <= 3.4028234e38f)) outs |= 1u << (kp & 31);
           }
+          outs = __reduce_or_sync(0xffffffffu, outs);
+          if (lane == 0) odd[st * 2 * NC + kw] = outs;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(&full[st]);
       }
-    } else {
+    } else if (pw != 4) {
       // ---------------------------------------------------------- values
-      const int vw = role - 1;
+      const int vw = pw < 3 ? pw - 1 : pw - 4;
       bool ok = true;
       int e = 14, low = 255;
       // int8: eight positions (an octet) by VP / 8 dims a thread: a warp reads
@@ -818,9 +837,33 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
           }
         }
       };
-      if (I8 && nblk > 0) load(0);
+      // f32: VP / 4 lanes an octet, OCT octets at a time.
+      constexpr int OCT = 128 / VP, PASS = 2 / OCT;
+      float4 fn[8];
+      auto fetch = [&](int i, int p) {
+        const int v = (blk0 + i) * BN + (vw * 2 + p * OCT + lane % OCT) * 8, d = lane / OCT * 4;
+        if (P.plain((blk0 + i) * BN, BN)) {  // the same for the warp
+          const float* src = reinterpret_cast<const float*>(A.v) + P.row(v) * A.vh + d;
+          const size_t step = (size_t)A.kvh * A.vh;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            fn[j] = d < A.vh ? __ldg(reinterpret_cast<const float4*>(src + j * step)) : make_float4(0, 0, 0, 0);
+          return;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = v + j < P.total && d < A.vh;
+          const float* row =
+              reinterpret_cast<const float*>(P.in_draft(v + j) ? A.tv : A.v) + (in ? P.row(v + j) : 0) * A.vh + (in ? d : 0);
+          fn[j] = in ? __ldg(reinterpret_cast<const float4*>(row)) : make_float4(0, 0, 0, 0);
+        }
+      };
+      if (nblk > 0) {
+        if (I8) load(0);
+        else if (PASS == 1) fetch(0, 0);
+      }
       for (int i = 0; i < nblk; ++i) {
-        const int st = i % NST, v0 = (blk0 + i) * BN;
+        const int st = i % NST;
         unsigned char* vt = stages + (size_t)st * C::STAGE + C::PARTS * C::K_TILE;
         if (I8) {
           const int pr = lane & 7;
@@ -851,95 +894,97 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
             }
           }
         } else {
-          // f32: a warp holds 32 positions (four octets; of 128-wide values two
-          // at a time) whole, four dims a lane in each of two rounds, so a
-          // position's largest value is the warp's own matter. A value is scaled
-          // like a key; 2^(140 - e) is a step's share of the scale, by the largest
-          // exponent of both warps so far.
-          constexpr int OCT = VP == 64 ? 4 : 2, PASS = 4 / OCT, DR = 128 / OCT;
-          const int oc = lane % OCT;
-          auto at = [&](const float* row, int d) {
-            return row && d < A.vh ? __ldg(reinterpret_cast<const float4*>(row + d)) : make_float4(0, 0, 0, 0);
-          };
-          // Exponent field of each position's largest value (0 none, 255 not finite), a byte a position.
-          int top = 0, least = 255;
-          uint32_t ef[PASS][2], bad = 0;
+          // f32: a warp holds 16 positions (two octets; of 128-wide values one at a
+          // time) whole, four dims a lane, so a position's largest value is the
+          // warp's own matter. A value is scaled like a key; 2^(140 - e) is a step's
+          // share of the scale, by the largest exponent of the warps so far. Lanes
+          // take their four dims in an order that keeps their writes in different
+          // banks.
+          const int da = lane / OCT * 4, turn = OCT == 2 ? lane >> 1 & 2 : lane >> 1 & 3;
+          int top = 0, least = 255, own[2] = {0, 0};
+          uint32_t bad = 0;
+          int* seen = vmax + (i & 1) * 8;
 #pragma unroll
           for (int p = 0; p < PASS; ++p) {
-            const int pr = vw * 4 + p * OCT + oc, da = lane / OCT * 4;
-            float4 x[2][8];
+            const int pr = vw * 2 + p * OCT + lane % OCT;
+            float4 x[8];
+            if (PASS == 2) fetch(i, p);  // without registers to hold two
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = fn[j];
+            if (PASS == 1 && i + 1 < nblk) fetch(i + 1, 0);
+            // The octet's eight maxima, one left a lane: position lane / 4.
+            float a[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int vj = v0 + pr * 8 + j;
-              const float* row =
-                  vj < P.total ? reinterpret_cast<const float*>(P.in_draft(vj) ? A.tv : A.v) + P.row(vj) * A.vh : nullptr;
-              x[0][j] = at(row, da), x[1][j] = at(row, DR + da);
+              const float t = fabsf(x[j].x) + fabsf(x[j].y) + fabsf(x[j].z) + fabsf(x[j].w);  // NaN where one is
+              a[j] = fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
+              a[j] = t == t ? a[j] : INFINITY;
             }
-            ef[p][0] = ef[p][1] = 0;
+#pragma unroll
+            for (int h = 4; h >= 1; h >>= 1) {
+              const bool up = lane & 4 * h;
+#pragma unroll
+              for (int j = 0; j < h; ++j) {
+                const float send = up ? a[j] : a[j + h], keep = up ? a[j + h] : a[j];
+                a[j] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, 4 * h));
+              }
+            }
+#pragma unroll
+            for (int d = OCT; d < 4; d <<= 1) a[0] = fmaxf(a[0], __shfl_xor_sync(0xffffffffu, a[0], d));
+            // Its exponent field: 0 none, 255 not finite.
+            const int eb = (int)(__float_as_uint(a[0]) >> 23);
+            const int y = a[0] == 0.f ? 0 : eb == 255 ? 255 : min(max(eb, 14), 253);
+            if (p == 0) own[0] = y;
+            else own[1] = y;
+            if (y == 255) bad |= 1u << (8 * (pr & 1) + (lane >> 2));
+            if (y != 0 && y != 255) top = max(top, y - 13), least = min(least, y - 13);
+            if (p + 1 == PASS) {
+              top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
+              if (lane == 0) seen[vw] = top, seen[4 + vw] = least;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float4 f = x[0][j], g = x[1][j];
-              float a = fmaxf(fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))),
-                              fmaxf(fmaxf(fabsf(g.x), fabsf(g.y)), fmaxf(fabsf(g.z), fabsf(g.w))));
-              const float t = fabsf(f.x) + fabsf(f.y) + fabsf(f.z) + fabsf(f.w) + fabsf(g.x) + fabsf(g.y) + fabsf(g.z) +
-                              fabsf(g.w);  // NaN where one is
-              if (t != t) a = INFINITY;
-#pragma unroll
-              for (int d = OCT; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-              const int y = a == 0.f ? 0 : a <= 3.4028234e38f ? min(max((int)(__float_as_uint(a) >> 23), 14), 253) : 255;
-              if (y == 255) bad |= 1u << (8 * (p * OCT + oc) + j);
-              else if (y > 0) top = max(top, y - 13), least = min(least, y - 13);
-              ef[p][j >> 2] |= (uint32_t)y << (8 * (j & 3));
+              const int yj = __shfl_sync(0xffffffffu, y, 4 * j + lane % OCT);
+              const bool use = yj != 0 && yj != 255;  // nothing of one that is not finite
+              const float by = __uint_as_float((uint32_t)(267 - yj) << 23);
+              x[j] = use ? make_float4(x[j].x * by, x[j].y * by, x[j].z * by, x[j].w * by) : make_float4(0, 0, 0, 0);
+              if (OCT == 1 && turn & 1) x[j] = make_float4(x[j].y, x[j].z, x[j].w, x[j].x);
+              if (turn & 2) x[j] = make_float4(x[j].z, x[j].w, x[j].x, x[j].y);
             }
             if (p == 0) {
               if (ok && !mbar_wait_spin(&empty[st], ((uint32_t)(i / NST) & 1u) ^ 1u, abort, werr)) ok = false;
               __syncwarp();
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int d0 = h * DR + da;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int y = (int)((ef[p][j >> 2] >> (8 * (j & 3))) & 255u);
-                const bool use = y > 0 && y < 255;  // nothing of one that is not finite
-                const float by = __uint_as_float((uint32_t)(267 - (use ? y : 140)) << 23);
-                x[h][j].x = use ? x[h][j].x * by : 0.f, x[h][j].y = use ? x[h][j].y * by : 0.f;
-                x[h][j].z = use ? x[h][j].z * by : 0.f, x[h][j].w = use ? x[h][j].w * by : 0.f;
-              }
-              if (d0 >= A.vh) continue;
+            if (da < A.vh) {
 #pragma unroll
               for (int t = 0; t < 4; ++t) {
                 uint32_t hh[4], ll[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  const float4 a = x[h][2 * j], c = x[h][2 * j + 1];
+                  const float4 a = x[2 * j], c = x[2 * j + 1];
                   halves(t == 0 ? a.x : t == 1 ? a.y : t == 2 ? a.z : a.w, t == 0 ? c.x : t == 1 ? c.y : t == 2 ? c.z : c.w,
                          &hh[j], &ll[j]);
                 }
-                const int d = d0 + t;
+                const int d = da + ((t + turn) & 3);
                 unsigned char* to = vt + d * 128 + ((pr ^ (d & 7)) << 4);
                 *reinterpret_cast<uint4*>(to) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
                 *reinterpret_cast<uint4*>(to + C::V_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
               }
             }
           }
-          top = __reduce_max_sync(0xffffffffu, top), least = __reduce_min_sync(0xffffffffu, least);
           bad = __reduce_or_sync(0xffffffffu, bad);
-          if (lane == 0) vmax[(i & 1) * 4 + vw] = top, vmax[(i & 1) * 4 + 2 + vw] = least;
-          asm volatile("bar.sync 4, 64;" ::: "memory");
-          e = max(e, max(vmax[(i & 1) * 4], vmax[(i & 1) * 4 + 1]));
-          low = min(low, min(vmax[(i & 1) * 4 + 2], vmax[(i & 1) * 4 + 3]));
-          if (lane == 0) odd[st * 2 * NC + NC + vw] = bad;
+          asm volatile("bar.sync 4, 128;" ::: "memory");
+          e = max(max(e, max(seen[0], seen[1])), max(seen[2], seen[3]));
+          low = min(min(low, min(seen[4], seen[5])), min(seen[6], seen[7]));
+          if (lane == 0) reinterpret_cast<uint16_t*>(odd + st * 2 * NC + NC)[vw] = (uint16_t)bad;
           if (vw == 0 && lane == 0) expo[2 * st] = e, expo[2 * st + 1] = low;
-          if (lane < OCT) {
+          if ((lane & 3) < OCT) {
 #pragma unroll
-            for (int p = 0; p < PASS; ++p)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int x = (int)((ef[p][j >> 2] >> (8 * (j & 3))) & 255u), f = 127 + x - e;  // 2^(x - 140) 2^(140 - e)
-                col_v[st * BN + (vw * 4 + p * OCT + oc) * 8 + j] =
-                    x > 0 && x < 255 && f > 0 ? __uint_as_float((uint32_t)f << 23) : 0.f;
-              }
+            for (int p = 0; p < PASS; ++p) {
+              const int y = own[p], f = 127 + y - e;  // 2^(y - 140) 2^(140 - e)
+              col_v[st * BN + (vw * 2 + p * OCT + lane % OCT) * 8 + (lane >> 2)] =
+                  y != 0 && y != 255 && f > 0 ? __uint_as_float((uint32_t)f << 23) : 0.f;
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1004,38 +1049,50 @@ cudaError_t launch_umma_form(const TreeArgs& A, int B, cudaStream_t st) {
   return cudaSuccess;
 }
 
-typedef TreeUmma<true, 3, 64, 4> UmmaI8x48;
-typedef TreeUmma<true, 4, 64, 4> UmmaI8x64;
-typedef TreeUmma<true, 8, 128, 4> UmmaI8x128;
-typedef TreeUmma<false, 3, 64, 2> UmmaF32x48;
-typedef TreeUmma<false, 4, 64, 2> UmmaF32x64;
-typedef TreeUmma<false, 8, 128, 2> UmmaF32x128;
+typedef TreeUmma<true, 3, 64, 1, 4> UmmaI8x48;
+typedef TreeUmma<true, 4, 64, 1, 4> UmmaI8x64;
+typedef TreeUmma<true, 8, 128, 2, 4> UmmaI8x128;
+typedef TreeUmma<false, 3, 64, 2, 5> UmmaF32x48;
+typedef TreeUmma<false, 4, 64, 2, 5> UmmaF32x64;
+typedef TreeUmma<false, 8, 128, 2, 2> UmmaF32x128;
 
 }  // namespace
 
 // More than 16 rows, whole 16-byte pieces and MMA steps. A step costs nearly the
 // same for 17 rows as for 128; mma.sync pays per 16 rows. Measured, mma.sync -> here:
-//   rows   48/64 int8, 256 x 1043   48/64 f32, 128 x 1043   128 int8, 4 x 16000   128 f32, 2 x 8000
+//   rows   48/64 int8, 256 x 1043   48/64 f32, 128 x 1043   128 int8, 4 x 16000   128 f32, 32 x 1043
 //    12        71 ->  63 us              68 ->  83 us            100 -> 111 us
-//    16                                                                              134 us -> (not taken)
-//    24       129 ->  64                114 ->  83               157 -> 112          220 -> 135
-//    48       127 ->  74                202 ->  85               251 -> 116          304 -> 136 (36 rows)
-//    96       192 ->  79                211 ->  90               383 -> 125          750 -> 150 (128 rows)
+//    24       129 ->  64                114 ->  83               157 -> 112          431 -> 184 us
+//    48       127 ->  74                202 ->  85               251 -> 116          688 -> 186 (64 rows)
+//    96       192 ->  79                211 ->  76               383 -> 125         1348 -> 199 (128 rows)
 // and at eight sessions of 1043 (48/64 int8) 12 rows 15 -> 19, 24 rows 21 -> 19.
 bool tree_umma_takes(int int8, int rows, int qk, int vh, int piece) {
   return piece == 16 && qk % 16 == 0 && vh % 16 == 0 && rows > 16;
 }
 
-// Splits that need the fewest rounds of blocks: a block of positions costs
-// about 1, a CTA's start and end about 4.
-int tree_umma_nsplit(int B, int rows, int kvh, int qk, int vh, int span) {
-  const bool wide = qk > 64 || vh > 64;
-  const long work = (long)B * kvh * ((rows + 127) / 128), room = 148 * (wide ? 1 : 2);
+// The cheapest number of position splits, in us: what a step of 64 positions
+// costs a block that has its SM to itself, or (int8 heads up to 64 wide) shares
+// it with another; a block's start and end, more where it leaves partial results;
+// their join. Measured (splits: us):
+//   int8 48/64: 256 x 96 rows x 1043    1: 78    2: 132   4: 160
+//               1 x 384 rows x 6000     1: 118   8: 30   16: 25   24: 24  32: 29  48: 31
+//   int8 128:   4 x 128 rows x 32771    1: 812   4: 230   9: 223  16: 268
+//               20 x 64 rows x 1043     1: 69    2: 83    4: 100
+//   f32 48/64:  16 x 288 rows x 2051    1: 66    2: 77    3: 67    6: 84
+//   f32 128:    2 x 128 rows x 8000     1: 511   4: 158   8: 105   9: 105  16: 119
+int tree_umma_nsplit(int int8, int B, int rows, int kvh, int qk, int vh, int span) {
+  const bool wide = qk > 64 || vh > 64, two = int8 && !wide;
+  const double one = int8 ? (wide ? 1.6 : 1.2) : (wide ? 3.8 : 1.9), both = two ? 2.1 : one;
+  const long work = (long)B * kvh * ((rows + 127) / 128), room = 148 * (two ? 2 : 1);
   const int blocks = (span + 63) / 64;
   int best = 1;
   double cost = 1e300;
   for (int ns = 1; ns <= 128 && ns <= blocks; ++ns) {
-    const double c = (double)((work * ns + room - 1) / room) * ((blocks + ns - 1) / ns + 4) + (ns > 1 ? 4.0 : 0.0);
+    const long rest = work * ns % room;
+    const double step = (blocks + ns - 1) / ns, ends = ns > 1 ? 13 : 6;
+    const double c = (double)(work * ns / room) * (both * step + ends) +
+                     (rest == 0 ? 0.0 : (rest <= 148 ? one : both) * step + ends) +
+                     (ns > 1 ? 3 + 1.9 * ((ns + 7) / 8) : 0.0);
     if (c < cost * 0.97) cost = c, best = ns;
   }
   return best;
