@@ -1062,9 +1062,9 @@ typedef TreeUmma<false, 8, 128, 2, 2> UmmaF32x128;
 // same for 17 rows as for 128; mma.sync pays per 16 rows. Measured, mma.sync -> here:
 //   rows   48/64 int8, 256 x 1043   48/64 f32, 128 x 1043   128 int8, 4 x 16000   128 f32, 32 x 1043
 //    12        71 ->  63 us              68 ->  83 us            100 -> 111 us
-//    24       129 ->  64                114 ->  83               157 -> 112          431 -> 184 us
-//    48       127 ->  74                202 ->  85               251 -> 116          688 -> 186 (64 rows)
-//    96       192 ->  79                211 ->  76               383 -> 125         1348 -> 199 (128 rows)
+//    24       129 ->  64                114 ->  69               157 -> 112          431 -> 184 us
+//    48       127 ->  74                202 ->  72               251 -> 116          688 -> 186 (64 rows)
+//    96       192 ->  78                211 ->  75               383 -> 125         1348 -> 199 (128 rows)
 // and at eight sessions of 1043 (48/64 int8) 12 rows 15 -> 19, 24 rows 21 -> 19.
 bool tree_umma_takes(int int8, int rows, int qk, int vh, int piece) {
   return piece == 16 && qk % 16 == 0 && vh % 16 == 0 && rows > 16;
