@@ -349,19 +349,20 @@ int nd_attend_tree(const float *q, int ldq, const void *k, const void *v, const 
                    const float *tks, const float *tvs, const uint32_t *mask, int B, int T, int heads,
                    int kv_heads, int qk, int vh, float *out, void *stream);
 
-/* Corrects logits [rows][ld] into out [rows][ldo] (out == logits: in place) and
- * picks each row's first maximum into picks [rows] (may be NULL). In order, for
- * row r: a token that occurs in hist[hist_off[r] .. hist_off[r + 1]) is divided
- * by repetition[r] when positive, else multiplied; one that occurs c > 0 times
- * from hist[gen_from[r]] on (NULL: in all of it) loses c * frequency[r] +
+/* Corrects logits [rows][ld] into out [rows][ldo] (out == logits with ldo == ld:
+ * in place; otherwise the two must not overlap) and picks each row's first
+ * maximum into picks [rows] (may be NULL). In order, for row r: a token that
+ * occurs in hist[hist_off[r] .. hist_off[r + 1]) is divided by repetition[r]
+ * when positive, else multiplied; one that occurs c > 0 times from
+ * hist[gen_from[r]] on (NULL: in all of it) loses c * frequency[r] +
  * presence[r] (c below 2^22); the biases of bias_ids[bias_off[r] ..
- * bias_off[r + 1]) are added, an id's summed in list order; a token whose bit (id % 32 of
- * mask[r * mask_ld + id / 32]) is clear becomes `masked` (the grammar mask of
- * needle_tokenizer_tool_mask uses -1e9; -INFINITY removes it from any
- * softmax). All arrays are device memory. hist, bias_ids and mask may each be
- * NULL: no token seen (the penalties then do nothing), no bias, no mask; so may
- * each penalty. Ids outside 0..vocab-1 are ignored. A
- * NaN is never picked; a row of -INFINITY or NaN alone picks 0. */
+ * bias_off[r + 1]) are added, an id's summed in list order; a token whose bit
+ * (id % 32 of mask[r * mask_ld + id / 32]) is clear becomes `masked` (the
+ * grammar mask of needle_tokenizer_tool_mask uses -1e9; -INFINITY removes it
+ * from any softmax). All arrays are device memory. hist, bias_ids and mask may
+ * each be NULL: no token seen (the penalties then do nothing), no bias, no mask;
+ * so may each penalty. Ids outside 0..vocab-1 are ignored. A NaN is never
+ * picked; a row of -INFINITY or NaN alone picks 0. */
 int nd_logits_adjust(const float *logits, int ld, int rows, int vocab, float *out, int ldo, const int *hist,
                      const int *hist_off, const int *gen_from, const float *repetition, const float *presence,
                      const float *frequency, const int *bias_ids, const float *bias_vals,

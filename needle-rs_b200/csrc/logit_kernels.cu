@@ -264,10 +264,19 @@ cudaError_t launch_logits_adjust(const float* x, int ldx, int rows, int vocab, f
   if (rows <= 0) return cudaSuccess;
   LogitArgs A{x, y, ldx, ldy, vocab, 0, 0, hist, hist_off, gen_from, rep, pres, freq,
               bias_ids, bias_vals, bias_off, mask, mask_ld, masked, picks};
-  // Blocks per row: one per 1024 ids, at most 8 (a portable cluster); each
-  // takes its share in equal chunks of at most LG_CHUNK ids.
+  // Blocks per row, at most 8 (a portable cluster), each with its share in equal
+  // chunks of at most LG_CHUNK ids: every one reads the row's history, so more
+  // only while SMs are free (two a SM of 1024 ids, four of 8192) or the turns
+  // become many. Measured (blocks: us):
+  //     8 x 8192     1: 10.0  2: 8.5   4: 8.3   8: 7.8
+  //    64 x 8192     1: 10.5  2: 8.5   4: 8.5   8: 9.7
+  //   256 x 8192     1: 10.5  2: 12.3  4: 16.6  8: 25.0
+  //    64 x 100003   1: 74.0  2: 40.9  4: 26.3  8: 20.8
+  //   256 x 100003   1: 112   2: 73.5  4: 73.7  8: 75.8
   int blocks = 1;
-  while (blocks < 8 && vocab > 1024 * blocks) blocks *= 2;
+  while (blocks < 8 && ((2l * rows * blocks <= 296 && vocab > 1024 * blocks) ||
+                        (2l * rows * blocks <= 592 && vocab > 8192 * blocks) || vocab > 2 * LG_CHUNK * blocks))
+    blocks *= 2;
   A.loops = (int)((vocab + (long)LG_CHUNK * blocks - 1) / ((long)LG_CHUNK * blocks));
   const long parts = (long)A.loops * blocks;
   A.chunk = (int)(((vocab + parts - 1) / parts + 3) / 4 * 4);

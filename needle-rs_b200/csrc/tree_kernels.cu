@@ -730,9 +730,29 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const float* __restrict_
 }
 
 template <bool I8, int QKP, int VHP, int MT>
+constexpr size_t tree_smem() {
+  return std::max((size_t)TREE_WARPS * TreeTile<I8, QKP, VHP>::WARP_BYTES,
+                  (size_t)(TREE_WARPS + 1) * MT * 16 * (VHP + 4) * 4);
+}
+
+// Blocks an SM holds.
+template <bool I8, int QKP, int VHP, int MT>
+int tree_resident() {
+  static const int n = [] {
+    auto kern = attend_tree_kernel<I8, QKP, VHP, MT>;
+    int r = 0;
+    if (allow_smem((const void*)kern, tree_smem<I8, QKP, VHP, MT>(), true) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&r, kern, TREE_THREADS, tree_smem<I8, QKP, VHP, MT>()) != cudaSuccess)
+      r = 1;
+    return std::max(r, 1);
+  }();
+  return n;
+}
+
+template <bool I8, int QKP, int VHP, int MT>
 cudaError_t launch_tree(TreeArgs A, int B, int piece, cudaStream_t st) {
   using TT = TreeTile<I8, QKP, VHP>;
-  const size_t smem = std::max((size_t)TREE_WARPS * TT::WARP_BYTES, (size_t)(TREE_WARPS + 1) * MT * 16 * (VHP + 4) * 4);
+  const size_t smem = tree_smem<I8, QKP, VHP, MT>();
   auto kern = attend_tree_kernel<I8, QKP, VHP, MT>;
   cudaError_t e = allow_smem((const void*)kern, smem, true);
   if (e != cudaSuccess) return e;
@@ -760,11 +780,28 @@ cudaError_t launch_tree(TreeArgs A, int B, int piece, cudaStream_t st) {
 
 int tree_tile_rows(int R, int qk, int vh) { return R <= 16 || qk > 64 || vh > 64 ? 16 : 32; }
 
+// F<I8, QKP, VHP, MT> of the mma.sync form that heads of these widths and R rows take.
+#define NB_TREE_FORM(CALL)                                       \
+  do {                                                           \
+    const bool one = tree_tile_rows(R, qk, vh) == 16;            \
+    if (qk > 64 || vh > 64) CALL(128, 128, 1);                   \
+    else if (qk > 48 && one) CALL(64, 64, 1);                    \
+    else if (qk > 48) CALL(64, 64, 2);                           \
+    else if (one) CALL(48, 64, 1);                               \
+    else CALL(48, 64, 2);                                        \
+  } while (0)
+
 }  // namespace
 
 // How a call runs: on tcgen05 or mma.sync, and over how many position splits.
-// mma.sync: enough blocks for about four a SM, each split at least 8 blocks of
-// 32 positions.
+// mma.sync: as many as keep the grid in one wave (clusters leave a few places
+// empty), each of at least 8 blocks of 32 positions; 9 to 16 are 8, which join
+// inside their cluster. Measured at one token, 6 rows of 48/64 int8 (splits: us):
+//   16 x 1000   2: 17.4  4: 14.0  8: 12.9      32 x 1000   2: 18.0  6: 14.8  8: 22.8
+//   64 x 1000   1: 20.9  2: 20.2  3: 18.7  4: 27.9
+//   256 x 1000  1: 44.3  2: 56.9               16 x 4000   8: 18.7  9: 22.9  16: 27.0
+//   1 x 6000    4: 28.9  8: 19.8  16: 18.7  24: 16.7
+// and with eight splits left to a join kernel 16 x 1000 takes 15.3, 16 x 4000 20.8.
 TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv, const float* out, int int8, int B,
                    int T, int heads, int kvh, int qk, int vh, int slots) {
   const int es = int8 ? 1 : 4, R = T * (heads / kvh);
@@ -779,8 +816,13 @@ TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv,
   }
   const int tr = tree_tile_rows(R, qk, vh);
   const long ctas = (long)B * kvh * ((R + tr - 1) / tr);
-  const long want = (592 + ctas - 1) / ctas, most = std::max(1, (slots + 255) / 256);
+  int res = 1;
+#define NB_RES(Q, V, M) res = int8 ? tree_resident<true, Q, V, M>() : tree_resident<false, Q, V, M>()
+  NB_TREE_FORM(NB_RES);
+#undef NB_RES
+  const long want = 148l * res * 12 / 13 / ctas, most = std::max(1, (slots + 255) / 256);
   P.nsplit = (int)std::max(1l, std::min(std::min(want, most), 256l));
+  if (P.nsplit > TREE_CLUSTER && P.nsplit <= 2 * TREE_CLUSTER) P.nsplit = TREE_CLUSTER;
   // Up to eight splits are a cluster that joins itself; more leave partial
   // results for a second kernel.
   P.part = P.nsplit > TREE_CLUSTER;
@@ -810,14 +852,9 @@ cudaError_t launch_attend_tree(const float* q, int ldq, const void* k, const voi
   const int piece = plan.piece;
   const int R = T * A.rep;
   cudaError_t e;
-  const bool one = tree_tile_rows(R, qk, vh) == 16;
 #define NB_TREE(Q, V, M) e = int8 ? launch_tree<true, Q, V, M>(A, B, piece, st) : launch_tree<false, Q, V, M>(A, B, piece, st)
   if (plan.umma) e = launch_tree_umma(A, int8, B, st);
-  else if (qk > 64 || vh > 64) NB_TREE(128, 128, 1);
-  else if (qk > 48 && one) NB_TREE(64, 64, 1);
-  else if (qk > 48) NB_TREE(64, 64, 2);
-  else if (one) NB_TREE(48, 64, 1);
-  else NB_TREE(48, 64, 2);
+  else NB_TREE_FORM(NB_TREE);
 #undef NB_TREE
   if (e != cudaSuccess || !plan.part) return e;
   const long rows = (long)B * T * heads;
