@@ -66,7 +66,7 @@ __device__ __forceinline__ float adjust(float x, uint32_t n, int id, float rep, 
 // bound it, the mask is one bit; the history costs 8 bytes per id and block.
 template <bool BIAS>
 __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitArgs A) {
-  extern __shared__ __align__(16) uint32_t cnt[];  // [chunk + 4], none without history and biases
+  extern __shared__ __align__(16) uint32_t cnt[];  // [chunk + 32], none without history and biases
   __shared__ unsigned long long best_of[LG_THREADS / 32];
   __shared__ unsigned long long of_rank[8];  // block 0 of a cluster: every block's best
   __shared__ __align__(16) int bid[BIAS ? LG_LIST : 4];
@@ -84,10 +84,10 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitArgs A
   const int* list = BIAS ? A.bias_ids + b0 : nullptr;
   const float* vals = BIAS ? A.bias_vals + b0 : nullptr;
   const bool marks = A.hist || BIAS;
-  // Row elements before the first 16-byte boundary of x; wide accesses need y
-  // to have as many.
-  const int skew = (int)(((uintptr_t)x >> 2) & 3);
-  const bool wide = skew == (int)(((uintptr_t)y >> 2) & 3);
+  // Row elements after the last 128-byte boundary before x, so that a warp's
+  // accesses are whole lines; wide ones need y on a 16-byte boundary with it.
+  const int skew = (int)(((uintptr_t)x >> 2) & 31);
+  const bool wide = (skew & 3) == (int)(((uintptr_t)y >> 2) & 3);
   float best = -INFINITY;
   int at = 0x7fffffff;
 
@@ -115,10 +115,10 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitArgs A
     load(tid);
     if (marks) {
       if (l) __syncthreads();
-      for (int i = tid; i < (A.chunk + 4) / 4; i += LG_THREADS) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i < (A.chunk + 32) / 4; i += LG_THREADS) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
       if (BIAS && l == 0 && tid < nb && nb <= LG_LIST) bid[tid] = list[tid], braw[tid] = vals[tid];
       __syncthreads();
-      // Shared index of id c0 + j is j + skew (chunks are multiples of 4, so the
+      // Shared index of id c0 + j is j + skew (chunks are multiples of 32, so the
       // wide accesses below are aligned in both).
       for (int i = h0 + tid; i < h1; i += LG_THREADS) {
         const uint32_t j = (uint32_t)A.hist[i] - (uint32_t)c0;
@@ -279,8 +279,8 @@ cudaError_t launch_logits_adjust(const float* x, int ldx, int rows, int vocab, f
     blocks *= 2;
   A.loops = (int)((vocab + (long)LG_CHUNK * blocks - 1) / ((long)LG_CHUNK * blocks));
   const long parts = (long)A.loops * blocks;
-  A.chunk = (int)(((vocab + parts - 1) / parts + 3) / 4 * 4);
-  const size_t smem = hist || bias_ids ? (size_t)(A.chunk + 4) * 4 : 0;
+  A.chunk = (int)(((vocab + parts - 1) / parts + 31) / 32 * 32);
+  const size_t smem = hist || bias_ids ? (size_t)(A.chunk + 32) * 4 : 0;
   auto kern = bias_ids ? logits_kernel<true> : logits_kernel<false>;
   cudaError_t e = allow_smem((const void*)kern, smem, true);
   if (e != cudaSuccess) return e;
