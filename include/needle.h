@@ -343,7 +343,8 @@ int nd_kv_read(const void *kc, const void *vc, const float *ks, const float *vs,
  * zeros, and what a node does not see never reaches its output, whatever it
  * holds. heads / kv_heads may be any number; qk and vh multiples of 4 up to 128;
  * T up to 4096. T = 1 is one decode step. Scores are scaled by 1 / sqrt(qk).
- * Partial results of long rings use stream-ordered scratch. */
+ * out must not overlap an input. Partial results of long rings use
+ * stream-ordered scratch. */
 int nd_attend_tree(const float *q, int ldq, const void *k, const void *v, const float *ks, const float *vs,
                    int int8, int slots, const int *lo, const int *hi, const void *tk, const void *tv,
                    const float *tks, const float *tvs, const uint32_t *mask, int B, int T, int heads,

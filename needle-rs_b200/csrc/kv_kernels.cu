@@ -30,7 +30,7 @@ __device__ __forceinline__ long ring_place(const int* sess, const int* pos, int 
 __device__ __forceinline__ bool superseded(const int* sess, const int* pos, int i, int M, const KvRing& R) {
   if (i >= M - R.slots || !sess) return false;
   const int j = i + R.slots;
-  return sess[j] == sess[i] && pos[j] == pos[i] + R.slots;
+  return sess[j] == sess[i] && pos[j] >= R.slots && pos[j] - R.slots == pos[i];
 }
 
 __device__ __forceinline__ uint32_t pack_codes(int a, int b, int c, int d) {

@@ -6,11 +6,14 @@ with long bias lists and vocabularies of several turns; two host threads.
 Tolerances are those of the 64-bit references (Tree.want, LOGIT_TOL), derived
 there.
 """
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
 import pytest
-from conftest import nb
+from conftest import ROOT, nb
 from test_gpu_draft import LOGIT_TOL, Tree, all_calls, dev, logits_ref, ptr, quant_ref
 
 pytestmark = pytest.mark.gpu
@@ -223,6 +226,25 @@ def test_append_of_special_vectors_equals_the_standalone_quantiser(cuda, d, vh):
         assert torch.equal(q, codes.reshape(M, n)), torch.nonzero(q != codes.reshape(M, n))[:4]
 
 
+def test_append_at_the_largest_positions(cuda):
+    """A row near the last position keeps its place: the row a ring's length
+    behind it in the call is skipped, not its successor."""
+    torch = cuda
+    M, slots = 9, 8
+    x = torch.randn(M, 32, device="cuda")
+    pos = torch.full((M,), -1, dtype=torch.int32, device="cuda")
+    pos[0], pos[8] = 2147483644, -2147483644  # 8 apart modulo 2^32
+    sess = torch.zeros(M, dtype=torch.int32, device="cuda")
+    for int8 in (False, True):
+        dt = torch.int8 if int8 else torch.float32
+        kc, vc = (torch.zeros(1, slots, 1, 16, dtype=dt, device="cuda") for _ in range(2))
+        ks, vs = (torch.zeros(1, slots, 1, device="cuda") for _ in range(2)) if int8 else (None, None)
+        nb.kv_append(ptr(x), 32, ptr(x) + 64, 32, ptr(sess), ptr(pos), M, int8, 1, slots, 1, 16, 16, ptr(kc), ptr(vc),
+                     ptr(ks), ptr(vs))
+        want = quant_ref(x[:1, :16].cpu().numpy())[0] if int8 else x[:1, :16].cpu().numpy()
+        assert np.array_equal(kc[0, 2147483644 % slots].cpu().numpy(), want)
+
+
 # ------------------------------------------------------------------ logits
 @pytest.mark.parametrize("vocab,ld,ldo,off", [
     (33, 33, 33, 0), (120007, 120007, 120007, 0), (102401, 102404, 102402, 1), (250001, 250003, 250003, 3),
@@ -300,3 +322,37 @@ def test_two_threads_on_streams_of_their_own(cuda):
     assert not failed
     for (_, outs, _), w in zip(sets, want):
         assert all(torch.equal(a, b) for a, b in zip(outs, w))
+
+
+FIRST = """
+import sys
+sys.path.insert(0, "tests")
+import torch
+torch.cuda.init()
+from test_gpu_draft import all_calls, nb
+stream = torch.cuda.Stream()
+nb.attend_tree, eager = (lambda *a, **k: None), nb.attend_tree  # all_calls runs it once
+calls, outs, hold = all_calls(torch, 3)
+nb.attend_tree = eager
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=stream):
+    for f in calls:
+        f(stream.cuda_stream)
+for _ in range(3):
+    g.replay()
+torch.cuda.synchronize()
+got = [o.clone() for o in outs]
+for f in calls:
+    f(None)
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, outs)), "replay differs"
+print("ok")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured(cuda):
+    """No call needs an eager one before it."""
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=ROOT, capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, PYTHONPATH=os.path.join(ROOT, "tests")))
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-2000:]
