@@ -146,6 +146,41 @@ def test_many_rows_with_windows_and_empty_nodes(cuda, int8):
     assert np.all(c.check(torch) == 0.0)
 
 
+@pytest.mark.parametrize("shape", [(1, 4, 1, 128, 128, 5651), (2, 4, 1, 32, 32, 6007), (1, 12, 2, 48, 64, 9001),
+                                   (9, 4, 1, 128, 128, 5651), (4, 12, 2, 48, 64, 9001)])
+@pytest.mark.parametrize("int8", [False, True])
+def test_long_contexts_are_as_exact_as_32_bits(cuda, int8, shape):
+    """Sums over thousands of positions lose no more than the same sums in plain
+    32-bit products and additions: nothing is left to accumulators that truncate."""
+    torch = cuda
+    T, heads, kvh, qk, vh, ctx = shape
+    c = Tree(1, T, heads, kvh, qk, vh, ctx, ctx, int8, seed=ctx)
+    c.lo[:] = 0
+    c.hi[:] = ctx - 1
+    c.mask[:] = 0
+    got = c.run(torch).cpu().numpy()[0]
+    k, v = c.k[0].astype(np.float64), c.v[0].astype(np.float64)
+    if int8:
+        k, v = k * c.ks[0][..., None], v * c.vs[0][..., None]
+    q = c.q[0, :, : heads * qk].reshape(T, heads, qk)
+
+    def attend(dt):
+        out = np.zeros((T, heads, vh), dt)
+        for h in range(heads):
+            kh, vv = k[:, h // (heads // kvh)].astype(dt), v[:, h // (heads // kvh)].astype(dt)
+            s = torch.from_numpy(q[:, h].astype(dt)).cuda() @ torch.from_numpy(kh).cuda().T / np.sqrt(qk)
+            w = torch.exp(s - s.max(-1, keepdim=True).values)
+            out[:, h] = (w @ torch.from_numpy(vv).cuda() / w.sum(-1, keepdim=True)).cpu().numpy()
+        return out
+
+    old = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    want, plain = attend(np.float64), attend(np.float32)
+    torch.backends.cuda.matmul.allow_tf32 = old
+    far = lambda x: float(np.linalg.norm(x - want) / np.linalg.norm(want))  # noqa: E731
+    assert far(got) <= max(1.5 * far(plain), 2.0 ** -20), (far(got), far(plain))
+
+
 @pytest.mark.parametrize("int8", [False, True])
 def test_outputs_at_any_float(cuda, int8):
     """An output start that is 4-byte aligned only, guarded on both sides."""
