@@ -1061,11 +1061,11 @@ typedef TreeUmma<false, 8, 128, 2, 2> UmmaF32x128;
 // More than 16 rows, whole 16-byte pieces and MMA steps. A step costs nearly the
 // same for 17 rows as for 128; mma.sync pays per 16 rows. Measured, mma.sync -> here:
 //   rows   48/64 int8, 256 x 1043   48/64 f32, 128 x 1043   128 int8, 4 x 16000   128 f32, 32 x 1043
-//    12        71 ->  63 us              68 ->  83 us            100 -> 111 us
-//    24       129 ->  64                114 ->  69               157 -> 112          431 -> 184 us
-//    48       127 ->  74                202 ->  72               251 -> 116          688 -> 186 (64 rows)
-//    96       192 ->  78                211 ->  75               383 -> 125         1348 -> 199 (128 rows)
-// and at eight sessions of 1043 (48/64 int8) 12 rows 15 -> 19, 24 rows 21 -> 19.
+//    12        53 ->  62 us              66 ->  68 us            89 -> 128 us         226 -> 189 us
+//    24        72 ->  63                 84 ->  69              155 -> 130            424 -> 188
+//    48       135 ->  75                156 ->  72              268 -> 133            627 -> 190
+//    96       204 ->  78                228 ->  75              522 -> 137           1159 -> 198
+// and at eight sessions of 1043 (48/64 int8) 12 rows 15.8 -> 17.2, 24 rows 21.6 -> 17.5.
 bool tree_umma_takes(int int8, int rows, int qk, int vh, int piece) {
   return piece == 16 && qk % 16 == 0 && vh % 16 == 0 && rows > 16;
 }
