@@ -186,7 +186,7 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeArgs& A, size_t node_at,
   const int o = A.drafted - v0;  // ring offset 0 is bit o
   if (o < 32) {
     w |= bit_range(o + start, o + min(start + cnt, n_ring));
-    if (start + cnt > A.slots) w |= bit_range(o, o + (start + cnt - A.slots));
+    if (start + cnt > A.slots) w |= bit_range(o, (int)((uint32_t)o + start + cnt - A.slots));  // the sum may pass 2^31
   }
   return w;
 }
