@@ -17,7 +17,8 @@
 // they accumulate, always towards zero: so a block's products start from zero,
 // remainders first, and are added to the running outputs (and long dot products
 // chunk by chunk) in f32. Left in the accumulators over 5651 positions the bias
-// was 8e-7 of the result against 4e-7 of the plain 32-bit form.
+// was 8e-7 of the result against 4e-7 of the plain 32-bit form. Eight sessions'
+// single token over 512 positions take 12 us: latency, 64 blocks of a short chain.
 #include <cooperative_groups.h>
 
 #include <algorithm>

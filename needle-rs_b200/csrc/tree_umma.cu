@@ -28,6 +28,12 @@
 // int8 heads of up to 64 leave room for two blocks on an SM, which hide each
 // other's latencies; the others take a whole SM.
 //
+// Measured: 256 sessions x 96 rows x 1043 int8 positions (48/64) 77 us (0.9 TB/s,
+// 20 % of the tensor pipe); 16 x 288 rows x 2051 f32 positions 65 us; 4 x 8 heads x
+// 128 rows x 32771 int8 positions (128 wide) 219 us (1.1 TB/s, 28 %). The chain of a
+// softmax step bounds the int8 forms: about 2900 cycles alone, 4300 with two blocks
+// on the SM, no pipe above 40 %.
+//
 // Every wait is bounded as in umma_gemm.cu.
 #include <algorithm>
 
