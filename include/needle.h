@@ -316,9 +316,13 @@ int nd_rope(const float *x, int ldx, float *y, int ldy, const int *pos, int M, i
  * each head vector as nd_kv_quant does, bit for bit. A row of negative position
  * or of a session outside 0..sessions-1 is skipped (a rejected or padding
  * row). No two rows of a call may name the same session and slot, save one
- * case: a session's rows stand one after another with ascending positions and
- * pass the ring's length (a prompt longer than its ring), where the later
- * rows win. Head widths up to 256, any strides. */
+ * case: a session's rows stand one after another, their positions ascending by
+ * one, and pass the ring's length (a prompt longer than its ring), where the
+ * later rows win; rows skipped for their position may stand among them under
+ * the same session index. Gaps in such a run's positions are not covered: of two
+ * rows that name one slot across a gap, or in any other order, either may be
+ * left in it, for int8 with the other's scale. Head widths up to 256, any
+ * strides. */
 int nd_kv_append(const float *k, int ldk, const float *v, int ldv, const int *sess, const int *pos, int M,
                  int int8, int sessions, int slots, int kv_heads, int qk, int vh, void *kc, void *vc,
                  float *ks, float *vs, void *stream);

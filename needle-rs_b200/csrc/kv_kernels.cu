@@ -26,11 +26,29 @@ __device__ __forceinline__ long ring_place(const int* sess, const int* pos, int 
 }
 
 // A prompt longer than its ring: whether a later row of the same call takes
-// row i's place (consecutive rows of a session, see needle.h).
+// row i's place. The session's rows stand one after another with positions that
+// ascend by one (see needle.h), so that row holds position pos[i] + slots, and is
+// row i + slots but for rows skipped in between: the walk goes ahead by what a
+// position lacks (fewer rows cannot do) and over skipped rows eight at a time, to
+// the session's end. Anything but the later position itself leaves row i alone.
 __device__ __forceinline__ bool superseded(const int* sess, const int* pos, int i, int M, const KvRing& R) {
   if (i >= M - R.slots || !sess) return false;
-  const int j = i + R.slots;
-  return sess[j] == sess[i] && pos[j] >= R.slots && pos[j] - R.slots == pos[i];
+  const int s = sess[i];
+  const long want = (long)pos[i] + R.slots;
+  for (long j = (long)i + R.slots; j < M && sess[j] == s;) {
+    const int q = pos[j];
+    if (q >= 0) {
+      if (q >= want) return q == want;
+      j += want - q;
+      continue;
+    }
+    long hop = 8;  // to the next row of the eight that is not skipped
+#pragma unroll
+    for (int u = 7; u >= 1; --u)
+      if (j + u < M && (sess[j + u] != s || pos[j + u] >= 0)) hop = u;
+    j += hop;
+  }
+  return false;
 }
 
 __device__ __forceinline__ uint32_t pack_codes(int a, int b, int c, int d) {
