@@ -300,8 +300,11 @@ typedef struct {
  * by side, at position pos[i] (device). The first rot_dim values of a head are
  * rotated, the rest copied: pair j is (j, j + rot_dim / 2), or (2j, 2j + 1)
  * when interleaved, turned by pos * theta^(-2j / rot_dim) (scaled as `scaling`
- * says; NULL: plain); `inverse` turns back. Angles are formed and reduced in 64
- * bits. Rows of negative position are left alone. rot_dim even, at most 256.
+ * says; NULL: plain). `inverse` turns by the negative angle with the same factor
+ * of cos and sin: the transpose, which takes the gradient of y to that of x. It
+ * gives x back where that factor m is 1, else m^2 x; with mscale = 1 / m it takes
+ * a rotation out of stored keys. Angles are formed and reduced in 64 bits. Rows
+ * of negative position are left alone. rot_dim even, at most 256.
  * Query and key heads that lie side by side in a projection's rows take one
  * call. The engine's own rotation (v3/model.rs:378-413) is the half layout over
  * the whole head. */

@@ -538,7 +538,9 @@ class RopeScaling(C.Structure):
 
 def rope(x_ptr, ldx, y_ptr, ldy, pos_ptr, M, heads, head_dim, rot_dim=None, theta=10000.0, interleaved=False,
          scaling=None, inverse=False, stream=None):
-    """Rotary positions of M rows of heads; y_ptr == x_ptr works in place."""
+    """Rotary positions of M rows of heads; y_ptr == x_ptr works in place.
+    inverse: the transpose (a gradient's way back). It undoes a rotation whose
+    scaling has a factor m on cos and sin when given mscale = 1 / m."""
     _check(lib().nd_rope(x_ptr, ldx, y_ptr, ldy, pos_ptr, M, heads, head_dim,
                          head_dim if rot_dim is None else rot_dim, theta, interleaved,
                          None if scaling is None else C.byref(scaling), inverse, stream), "nd_rope")

@@ -17,7 +17,7 @@ namespace nb {
 struct RopeFreqs {
   double turns[ROPE_MAX_ROT / 2];
   float m;    // factor of cos and sin
-  float sgn;  // -1 rotates back
+  float sgn;  // -1: the transpose, by the negative angle and the same m
 };
 
 // One block: `tok` tokens. Its threads first form the tokens' cosines and sines

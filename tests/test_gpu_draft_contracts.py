@@ -7,9 +7,69 @@ where nothing else stands beside the comparison.
 import numpy as np
 import pytest
 from conftest import nb
-from test_gpu_draft import dev, ptr, quant_ref
+from test_gpu_draft import ROPE_TOL, dev, ptr, quant_ref, rope_ref
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ the way back of a rotation
+SCALINGS = [(None, 1.0), (("linear", 4.0, 0), 1.0), (("by_parts", 32.0, 4096.0), 0.1 * np.log(32.0) + 1.0)]
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("scaling,m", SCALINGS)
+def test_rope_and_its_inverse_return_x(cuda, inter, scaling, m):
+    """Taking a rotation out again: with mscale = 1 / m the rows come back."""
+    torch = cuda
+    M, heads, dim, rot = 300, 3, 64, 48
+    rng = np.random.default_rng(4)
+    x = rng.normal(size=(M, heads * dim)).astype(np.float32)
+    pos = dev(torch, rng.integers(0, 1 << 20, M).astype(np.int32))
+    y = dev(torch, x)
+    for inverse in (False, True):
+        sc = None
+        if scaling is not None:
+            sc = nb.RopeScaling(scaling[0], scaling[1], trained=scaling[2], mscale=1.0 / m if inverse else 0.0)
+        nb.rope(ptr(y), heads * dim, ptr(y), heads * dim, ptr(pos), M, heads, dim, rot_dim=rot, interleaved=inter,
+                scaling=sc, inverse=inverse)
+    _, size = rope_ref(x, pos.cpu().numpy(), heads, dim, rot, 10000.0, inter, None, False)
+    # With e = ROPE_TOL (|x1| + |x2|): the rotation's errors, at most m e each, are both turned
+    # back and divided by m: 2 e. The way back adds its own bound of the rotated pair,
+    # ROPE_TOL (|y1| + |y2|) / m, at most sqrt(2) e. 1 / m is rounded once.
+    assert np.all(np.abs(y.cpu().numpy() - x) <= (2 + 2 ** 0.5) * ROPE_TOL * size + 2.0 ** -24 * np.abs(x))
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("scaling,m", SCALINGS)
+def test_rope_inverse_is_the_transpose(cuda, inter, scaling, m):
+    """The gradient's way back: <rope(x), g> = <x, inverse(g)> of every pair, by
+    the 64-bit rotation and by differences of it."""
+    torch = cuda
+    M, heads, dim, rot = 40, 2, 32, 24
+    rng = np.random.default_rng(5)
+    x, g = (rng.normal(size=(M, heads * dim)) for _ in range(2))
+    g = g.astype(np.float32)
+    pos = rng.integers(0, 1 << 20, M).astype(np.int32)
+    sc = None if scaling is None else nb.RopeScaling(scaling[0], scaling[1], trained=scaling[2])
+    gd, pd = dev(torch, g), dev(torch, pos)
+    out = torch.zeros(M, heads * dim, device="cuda")
+    nb.rope(ptr(gd), heads * dim, ptr(out), heads * dim, ptr(pd), M, heads, dim, rot_dim=rot, interleaved=inter,
+            scaling=sc, inverse=True)
+    got = out.cpu().numpy()
+
+    def rotated(a):
+        return rope_ref(a, pos, heads, dim, rot, 10000.0, inter, scaling, False)[0]
+
+    _, size = rope_ref(g, pos, heads, dim, rot, 10000.0, inter, scaling, False)
+    for d in range(dim):  # one value of every head and row at a time; the map is linear
+        step = np.zeros((M, heads, dim))
+        step[:, :, d] = 0.5
+        step = step.reshape(M, -1)
+        diff = (rotated(x + step) - rotated(x - step)) * g
+        want = diff.reshape(M, heads, dim).sum(-1)
+        # the differences' own rounding in 64 bits: below 2^-44 of values below 100
+        tol = ROPE_TOL * size.reshape(M, heads, dim)[:, :, d] + 2.0 ** -40
+        assert np.all(np.abs(got.reshape(M, heads, dim)[:, :, d] - want) <= tol)
 
 
 # ------------------------------------------------------------------ prompts longer than their rings
