@@ -351,7 +351,8 @@ int nd_kv_read(const void *kc, const void *vc, const float *ks, const float *vs,
  * holds. heads / kv_heads may be any number; qk and vh multiples of 4 up to 128;
  * T up to 4096. T = 1 is one decode step. Scores are scaled by 1 / sqrt(qk).
  * out must not overlap an input. Partial results of long rings use
- * stream-ordered scratch. */
+ * stream-ordered scratch. Rows left NaN by a wait that gave up are told by
+ * nd_take_wait_error below. */
 int nd_attend_tree(const float *q, int ldq, const void *k, const void *v, const float *ks, const float *vs,
                    int int8, int slots, const int *lo, const int *hi, const void *tk, const void *tv,
                    const float *tks, const float *tvs, const uint32_t *mask, int B, int T, int heads,
@@ -376,6 +377,20 @@ int nd_logits_adjust(const float *logits, int ld, int rows, int vocab, float *ou
                      const float *frequency, const int *bias_ids, const float *bias_vals,
                      const int *bias_off, const uint32_t *mask, int mask_ld, float masked, uint32_t *picks,
                      void *stream);
+
+/* Waits that gave up. The tcgen05 kernels (nd_cq_project and
+ * nd_cq_project_grouped on path 3, which path 0 takes for M > 8; nd_attend_tree
+ * with more than 16 rows of a KV head) wait inside a block, each wait bounded to
+ * about a second. Should one give up, its kernel raises a flag of the current device and
+ * its outputs are not to be used (nd_attend_tree writes NaN to the rows
+ * concerned); the call that launched it has returned 0 by then.
+ * nd_take_wait_error reads the flag into *gave_up (1: raised since it was last
+ * taken) and clears it; call it after synchronising with the streams of the
+ * calls in question, not during a capture. nd_wait_flag gives the flag's device
+ * address (one int, 0 or 1) to a caller that would rather copy it to the host
+ * beside its results, on its own stream or in a graph. */
+int nd_take_wait_error(int *gave_up);
+int nd_wait_flag(int **flag);
 
 /* Returns the cudaError_t of the last nd_* failure on this thread as text. */
 const char *nd_last_error(void);

@@ -157,6 +157,8 @@ def lib() -> C.CDLL:
                            [vp, vp]),
         "nd_logits_adjust": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, C.c_int] + [vp] * 10 +
                              [C.c_int, C.c_float, vp, vp]),
+        "nd_take_wait_error": (C.c_int, [C.POINTER(C.c_int)]),
+        "nd_wait_flag": (C.c_int, [C.POINTER(C.c_void_p)]),
         "nd_last_error": (C.c_char_p, []),
     }
     for name, (res, args) in sig.items():
@@ -519,6 +521,22 @@ def attend_step(q_ptr, k_ptr, v_ptr, ks_ptr, vs_ptr, int8, slots, lo_ptr, hi_ptr
                 qk, vh, out_ptr, stream=None):
     _check(lib().nd_attend_step(q_ptr, k_ptr, v_ptr, ks_ptr, vs_ptr, int(int8), slots, lo_ptr, hi_ptr, B,
                                 heads, kv_heads, qk, vh, out_ptr, stream), "nd_attend_step")
+
+
+def take_wait_error() -> bool:
+    """Whether a tensor-core kernel on the current device has given up a bounded
+    wait (its outputs are not to be used) since the last call; clears the flag.
+    Synchronise with the calls in question first."""
+    v = C.c_int(0)
+    _check(lib().nd_take_wait_error(C.byref(v)), "nd_take_wait_error")
+    return v.value != 0
+
+
+def wait_flag() -> int:
+    """Device address of that flag (one int32, 0 or 1)."""
+    p = C.c_void_p()
+    _check(lib().nd_wait_flag(C.byref(p)), "nd_wait_flag")
+    return p.value
 
 
 # ------------------------------------------------------------ drafted tokens

@@ -1225,6 +1225,16 @@ int nd_logits_adjust(const float* logits, int ld, int rows, int vocab, float* ou
                                             picks, (cudaStream_t)stream));
 }
 
+int nd_take_wait_error(int* gave_up) {
+  if (!gave_up) return nd_refuse("nd_take_wait_error: null pointer");
+  return nd_status(nb::umma_take_error(gave_up));
+}
+
+int nd_wait_flag(int** flag) {
+  if (!flag) return nd_refuse("nd_wait_flag: null pointer");
+  return nd_status(nb::umma_error_ptr(flag));
+}
+
 const char* nd_last_error(void) { return g_nd_err.c_str(); }
 
 }  // extern "C"

@@ -116,9 +116,9 @@ cudaError_t umma_cache_levels(CqMat* W, std::vector<void*>* owned, cudaStream_t 
 int cq_launches(const CqMat& W, int M, const GemmScratch* gs, int force_path = 0, bool presplit = false);
 cudaError_t cq_project_umma(const CqMat& W, const float* xh, int ldx, int M, float* y, int ldy, int row0,
                             int nrows, cudaStream_t st, const GemmScratch& gs, bool presplit = false);
-// Reads and clears the library-wide device flag raised when a bounded wait of
-// the tensor-core GEMM expired and the caller gave no flag of its own
-// (GemmScratch::werr null) (*flag != 0).
+// Reads and clears the library-wide device flag (*flag 0 or 1) raised when a
+// bounded wait expired in the tree attention, or in the tensor-core GEMM where
+// the caller gave no flag of its own (GemmScratch::werr null). nd_take_wait_error.
 cudaError_t umma_take_error(int* flag);
 // Device address of that library-wide flag on the current device.
 cudaError_t umma_error_ptr(int** p);

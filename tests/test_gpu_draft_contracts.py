@@ -7,9 +7,48 @@ where nothing else stands beside the comparison.
 import numpy as np
 import pytest
 from conftest import nb
-from test_gpu_draft import ROPE_TOL, dev, ptr, quant_ref, rope_ref
+from test_gpu_draft import ROPE_TOL, Tree, dev, ptr, quant_ref, rope_ref
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ waits that gave up
+class _Word:
+    """One int32 of device memory as torch takes it."""
+
+    def __init__(self, address):
+        self.__cuda_array_interface__ = dict(shape=(1,), typestr="<i4", data=(address, False), version=2)
+
+
+def test_a_wait_that_gave_up_is_told_once(cuda):
+    """The flag the kernels raise, raised here from outside: read, then clear.
+    Calls that wait as they should leave it alone."""
+    torch = cuda
+    Tree(2, 20, 4, 2, 48, 64, 90, 80, True, seed=1).check(torch)
+    torch.cuda.synchronize()
+    assert not nb.take_wait_error()
+    flag = torch.as_tensor(_Word(nb.wait_flag()), device="cuda")
+    flag.fill_(1)
+    torch.cuda.synchronize()
+    Tree(2, 20, 4, 2, 48, 64, 90, 80, True, seed=1).check(torch)  # no call clears or minds it
+    torch.cuda.synchronize()
+    assert nb.take_wait_error() and not nb.take_wait_error()
+    assert int(flag[0]) == 0
+
+
+def test_the_wait_flag_may_be_copied_in_a_graph(cuda):
+    torch = cuda
+    flag = torch.as_tensor(_Word(nb.wait_flag()), device="cuda")
+    seen = torch.zeros(1, dtype=torch.int32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        seen.copy_(flag)
+    for v in (0, 1):
+        flag.fill_(v)
+        g.replay()
+        torch.cuda.synchronize()
+        assert int(seen[0]) == v
+    assert nb.take_wait_error() and not nb.take_wait_error()
 
 
 # ------------------------------------------------------------------ the way back of a rotation
