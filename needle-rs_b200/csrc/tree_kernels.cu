@@ -150,6 +150,36 @@ __device__ __forceinline__ void tree_copy(char* buf, const char* k, const char* 
   }
 }
 
+// Row rr of KV head kh again over one warp's blocks of PB positions (blk0, blk0 +
+// TREE_WARPS .. below blk1; the ring's blocks first) in plain f32, into `row`:
+// outputs, and its max and sum at [at], [at + 1].
+template <bool I8>
+__device__ __noinline__ void tree_again(const TreeArgs& A, int b, int kh, int rr, int base, int n_ring, int PB,
+                                        int ring_blocks, int blk0, int blk1, float* row, int at) {
+  TreePlace P;
+  P.ring = (size_t)b * A.slots * A.kvh + kh, P.draft = (size_t)b * A.T * A.kvh + kh;
+  P.drafted = A.drafted, P.slot0 = base % A.slots, P.slots = A.slots, P.kvh = A.kvh, P.total = A.drafted + n_ring;
+  const int node = A.by_rep.div(rr), head = kh * A.rep + rr - node * A.rep, lane = threadIdx.x & 31;
+  const size_t node_at = (size_t)b * A.T + node;
+  const int h = A.hi[node_at];
+  int l = max(A.lo[node_at], 0);
+  if (h >= 0) l = max(l, h - A.slots + 1);
+  const int cnt = l <= h ? h - l + 1 : 0, start = cnt ? (int)((long)(l - base) % A.slots) : 0;
+  const float* q = A.q + node_at * A.ldq + (size_t)head * A.qk;
+  bool none = false;
+  for (int i = lane; i < A.qk; i += 32) none |= q[i] != q[i];
+  if (__any_sync(0xffffffffu, none)) return;  // a NaN in the query: NaN it stays
+  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int blk = blk0; blk < blk1; blk += TREE_WARPS) {
+    const int v0 = blk < ring_blocks ? P.drafted + blk * PB : (blk - ring_blocks) * PB;
+    tree_slow_row<I8>(A, P, node_at, node, head, start, cnt, n_ring, v0,
+                      min(v0 + PB, blk < ring_blocks ? P.total : P.drafted), &m, &sum, o);
+  }
+  for (int j = 0; j < 4; ++j)
+    if (lane + 32 * j < A.vh) row[lane + 32 * j] = o[j];
+  if (lane == 0) row[at] = m, row[at + 1] = sum;
+}
+
 // Grid (row tiles * kvh * nsplit, B), four warps: each holds the same MT * 16
 // rows (queries in registers) and takes every fourth block of PB positions of
 // its split through its own double-buffered copies, so the loop has no block
@@ -157,7 +187,7 @@ __device__ __forceinline__ void tree_copy(char* buf, const char* k, const char* 
 // the ring's (offsets 0 .. n_ring - 1 from the tile's lowest position) and
 // then the draft's nodes.
 template <bool I8, int QKP, int VHP, int MT>
-__global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const TreeArgs A, int piece, int cluster) {
+__global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const __grid_constant__ TreeArgs A, int piece, int cluster) {
   using TT = TreeTile<I8, QKP, VHP>;
   constexpr int PB = TT::PB, NT = PB / 8;        // 8-position score tiles of a block
   constexpr int KC = QKP / 16, VN = VHP / 8;     // 16-dim chunks of a key, 8-dim tiles of an output
@@ -319,6 +349,7 @@ __global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const TreeArg
   float o[MT][VN][4], mx[2 * MT], sum[2 * MT];
   int vexp, vlow;         // int8: outputs are held times 2^(140 - vexp); least exponent of a value scale
   bool careful = false;   // a second run over the blocks, see below
+  bool far = false;       // int8: a score may have passed the range
 again:
   vexp = 14, vlow = 255;
 #pragma unroll
@@ -479,6 +510,7 @@ again:
     float grow = 1.f;
     float2 v2[NT];
     if (I8) {
+      far |= fabsf(sc[lane]) > 0x1p96f;  // times a product of up to 2^28
       const uint32_t a = __float_as_uint(fabsf(sc[PB + lane]));
       const uint32_t top = __reduce_max_sync(0xffffffffu, a);
       vlow = min(vlow, (int)(__reduce_min_sync(0xffffffffu, a ? a : 0x7f800000u) >> 23));
@@ -607,10 +639,10 @@ again:
   }
   cp_wait<0>();
   // A weight of zero times a value that is no number must not count (a node
-  // masked for some rows only may hold anything), and neither may a scale that
-  // a row does not see cost it bits: where an output came out infinite or NaN,
-  // or the value scales lie more than 2^12 apart, the warp takes its blocks
-  // again, position by position in f32.
+  // masked for some rows only may hold anything), and neither may a scale that a
+  // row does not see cost it bits: where an output came out infinite or NaN, or
+  // the value scales lie more than 2^12 apart, the warp takes its blocks again,
+  // position by position in f32.
   if (!careful) {
     bool odd = I8 && vexp - vlow > 12;
 #pragma unroll
@@ -633,10 +665,12 @@ again:
 #pragma unroll
       for (int n = 0; n < VN; ++n) o[m][n][0] *= f, o[m][n][1] *= f, o[m][n][2] *= f, o[m][n][3] *= f;
   }
+  bool lost = far;
 #pragma unroll
   for (int i = 0; i < 2 * MT; ++i) {
     sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
     sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+    lost |= !(sum[i] <= 3.4028234e38f);
   }
   // ---- the four warps' results meet (shared memory reused)
   __syncthreads();
@@ -650,6 +684,20 @@ again:
 #pragma unroll
       for (int e = 0; e < 2; ++e) row[tree_dim<I8>(n, 2 * t + e)] = o[i >> 1][n][(i & 1) * 2 + e];
     if (t == 0) row[VHP] = mx[i], row[VHP + 1] = sum[i];
+  }
+  // Rows whose sum is no number (an infinite key has no finite parts: its
+  // remainder is NaN, but its score may be -inf and weigh nothing) are done again,
+  // and so is every row where a score may have passed the range before the query's
+  // power of two is taken back.
+  if (__any_sync(0xffffffffu, lost)) {
+    __syncwarp();
+    far = __any_sync(0xffffffffu, far);
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      float* row = P + ((size_t)wid * MT * 16 + r) * PW;
+      if (far || !(row[VHP + 1] <= 3.4028234e38f))
+        tree_again<I8>(A, b, kh, r0 + r, base, n_ring, PB, ring_blocks, blk0, blk1, row, VHP);
+    }
   }
   __syncthreads();
   // Splits of a cluster: each block leaves its rows (outputs, max, sum) in warp

@@ -8,7 +8,8 @@
 // operand of the second product. f32 accuracy from f16 operands: the query and
 // P are f16 high parts and remainders (22 bits; int8 codes are f16 values
 // exactly; f32 keys and values are split the same way after a power-of-two
-// scale per position, which is then treated like an int8 scale). The products
+// scale per position, which is then treated like an int8 scale; an element far
+// below its vector's largest is held to 2^-38 of that, where f16 ends). The products
 // with remainders go first: the tensor cores truncate when they accumulate,
 // and truncation costs only what the sum already holds. For the same reason O
 // is drained into f32 registers after every block.
@@ -155,103 +156,6 @@ __device__ __forceinline__ void widen(uint32_t u, uint32_t* a, uint32_t* b) {
   *a = *reinterpret_cast<uint32_t*>(&x);
   *b = *reinterpret_cast<uint32_t*>(&y);
 }
-// Bits [a, b) of a 32-bit word.
-__device__ __forceinline__ uint32_t bit_range(int a, int b) {
-  const uint32_t hi = b >= 32 ? 0xffffffffu : b <= 0 ? 0u : (1u << b) - 1u;
-  const uint32_t lo = a >= 32 ? 0xffffffffu : a <= 0 ? 0u : (1u << a) - 1u;
-  return hi & ~lo;
-}
-
-// Where position v of a call lies: the draft's nodes come first, the ring's
-// offsets after them.
-struct TreePlace {
-  size_t ring, draft;  // first row (position * kvh + kh) of the session in each
-  int drafted, slot0, slots, kvh, total;
-  __device__ __forceinline__ bool in_draft(int v) const { return v < drafted; }
-  __device__ __forceinline__ size_t row(int v) const {
-    if (v < drafted) return draft + (size_t)v * kvh;
-    int s = slot0 + (v - drafted);
-    if (s >= slots) s -= slots;
-    return ring + (size_t)s * kvh;
-  }
-  // Whether positions v .. v + n - 1 are ring places one after another.
-  __device__ __forceinline__ bool plain(int v, int n) const {
-    const int s = slot0 + (v - drafted);
-    return v >= drafted && v + n <= total && (s + n <= slots || s >= slots);
-  }
-};
-
-// What row `node` sees of positions v0 .. v0 + 31.
-__device__ __forceinline__ uint32_t tree_sees(const TreeArgs& A, size_t node_at, int node, int start, int cnt,
-                                              int n_ring, int v0) {
-  uint32_t w = 0;
-  if (v0 < A.drafted) {
-    w = A.mask ? __ldg(A.mask + node_at * A.words + (v0 >> 5)) : bit_range(0, node - v0 + 1);
-    w &= bit_range(0, A.drafted - v0);
-  }
-  const int o = A.drafted - v0;  // ring offset 0 is bit o
-  if (o < 32) {
-    w |= bit_range(o + start, o + min(start + cnt, n_ring));
-    if (start + cnt > A.slots) w |= bit_range(o, (int)((uint32_t)o + start + cnt - A.slots));  // the sum may pass 2^31
-  }
-  return w;
-}
-
-// One row over positions [v0, v1) by a warp, in f32 from the cache itself: the
-// rows whose values or scales f16 operands cannot hold. Returns log2 max, sum,
-// and dims lane + 32 j of the output.
-template <bool I8>
-__device__ __noinline__ void tree_slow_row(const TreeArgs& A, const TreePlace& P, size_t node_at, int node, int head,
-                                           int start, int cnt, int n_ring, int v0, int v1, float* m_out, float* l_out,
-                                           float (&o)[4]) {
-  const int lane = threadIdx.x & 31;
-  const float* q = A.q + node_at * A.ldq + (size_t)head * A.qk;
-  float m = -INFINITY, l = 0.f;
-  o[0] = o[1] = o[2] = o[3] = 0.f;
-  for (int base = v0 & ~31; base < v1; base += 32) {
-    const int v = base + lane;
-    const bool on = v >= v0 && v < v1 && ((tree_sees(A, node_at, node, start, cnt, n_ring, base) >> lane) & 1);
-    float s = -INFINITY;
-    if (on) {
-      const size_t r = P.row(v);
-      const bool d = P.in_draft(v);
-      s = 0.f;
-      if (I8) {
-        const int8_t* k = (const int8_t*)(d ? A.tk : A.k) + r * A.qk;
-        const float sc = (d ? A.tks : A.ks)[r];
-        for (int i = 0; i < A.qk; ++i) s = fmaf(q[i], (float)k[i] * sc, s);
-      } else {
-        const float* k = (const float*)(d ? A.tk : A.k) + r * A.qk;
-        for (int i = 0; i < A.qk; ++i) s = fmaf(q[i], k[i], s);
-      }
-      s *= A.scale;
-    }
-    const float mn = fmaxf(m, warp_max(s));
-    const float mz = mn == -INFINITY ? 0.f : mn;
-    const float corr = ex2(m - mz), p = on ? ex2(s - mz) : 0.f;
-    m = mn;
-    l = l * corr + warp_sum(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] *= corr;
-    for (int i = 0; i < 32; ++i) {
-      const float w = __shfl_sync(0xffffffffu, p, i);
-      if (w == 0.f) continue;  // the same for every lane
-      const size_t r = P.row(base + i);
-      const bool d = P.in_draft(base + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = lane + 32 * j;
-        if (e >= A.vh) continue;
-        const float x = I8 ? (float)((const int8_t*)(d ? A.tv : A.v))[r * A.vh + e] * (d ? A.tvs : A.vs)[r]
-                           : ((const float*)(d ? A.tv : A.v))[r * A.vh + e];
-        o[j] = fmaf(w, x, o[j]);
-      }
-    }
-  }
-  *m_out = m;
-  *l_out = l;
-}
-
 // Grid (tiles of 128 rows * kvh * nsplit, sessions).
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __grid_constant__ TreeArgs A, int* werr) {
@@ -736,7 +640,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + 1) ^ (kp & 7)) << 4)) =
                   make_uint4(w[4], w[5], w[6], w[7]);
             }
-            sane[h] = fabsf(ksc[h]) <= 3.4028234e38f && fabsf(vsc[h]) <= 3.4028234e38f;
+            // A product of the scaled query is up to 2^28: key scales from 2^96 on could take it past the range.
+            sane[h] = fabsf(ksc[h]) <= 0x1p96f && fabsf(vsc[h]) <= 3.4028234e38f;
           }
           // Value scales, held so that the largest so far is in [2^13, 2^14).
           uint32_t top = 0, least = 0x7f800000u;
@@ -799,7 +704,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               *reinterpret_cast<uint4*>(at + C::K_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
             }
             if (lane % LK == 0) col_k[st * BN + kp] = v0 + kp < P.total ? __uint_as_float((uint32_t)(ef - 13) << 23) : 0.f;
-            if (!(mx <= 3.4028234e38f)) outs |= 1u << (kp & 31);
+            if (!(mx <= 0x1p96f)) outs |= 1u << (kp & 31);  // as for int8: scaled products are up to 2^35
           }
           outs = __reduce_or_sync(0xffffffffu, outs);
           if (lane == 0) odd[st * 2 * NC + kw] = outs;
@@ -1018,7 +923,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       int ll = max(A.lo[at2], 0);
       if (hh >= 0) ll = max(ll, hh - A.slots + 1);
       const int c2 = ll <= hh ? hh - ll + 1 : 0, s2 = c2 ? (int)((long)(ll - base) % A.slots) : 0;
-      float m2, l2, o2[4];
+      float m2 = -INFINITY, l2 = 0.f, o2[4] = {0.f, 0.f, 0.f, 0.f};
       tree_slow_row<I8>(A, P, at2, n2, h2, s2, c2, n_ring, blk0 * BN, min((blk0 + nblk) * BN, P.total), &m2, &l2, o2);
       float* dst = A.nsplit > 1 ? A.part + ((((size_t)b * A.kvh + kh) * A.nsplit + z) * R + q2) * (A.vh + 2)
                                 : A.out + (at2 * A.heads + h2) * A.vh;

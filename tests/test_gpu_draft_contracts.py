@@ -170,3 +170,59 @@ def test_rows_skipped_inside_a_prompt_longer_than_its_ring(cuda, int8, slots, va
         if int8:
             for a, w in zip(sc, scales):
                 assert np.array_equal(a.cpu().numpy(), w)
+
+
+# ------------------------------------------------------------------ keys that are not finite
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("T,heads,kvh,qk,vh", [(1, 4, 2, 48, 64), (2, 12, 2, 48, 64), (5, 4, 2, 128, 128),
+                                               (3, 3, 3, 20, 36), (9, 12, 2, 48, 64), (17, 4, 2, 128, 128)])
+def test_a_score_of_minus_infinity_weighs_nothing(cuda, int8, T, heads, kvh, qk, vh):
+    """A seen key that every query meets with a score of -inf has weight 0: the
+    answer is the one without it, in the ring and in the draft, whichever form runs."""
+    torch = cuda
+    c = Tree(2, T, heads, kvh, qk, vh, 90, 80, int8, seed=T)
+    first = c.q[:, :, : heads * qk].reshape(2, T, heads, qk)
+    first[..., 5] = np.abs(first[..., 5]) + 0.25       # a view: every query is positive there
+    at = [int(c.hi[b, 0] - 7) % 90 for b in range(2)]
+    want, tol = c.want()
+    for b in range(2):
+        c.hi[b], c.lo[b] = c.hi[b], c.hi[b] - 20
+    with_it = c.mask.copy()
+    c.mask &= ~np.uint32(1)                            # node 0 unseen, and the ring's place left out:
+    lo, hi = c.lo.copy(), c.hi.copy()
+    seen = c.seen
+    c.seen = lambda b, t: ([s for s in seen(b, t)[0] if s != at[b]], seen(b, t)[1])
+    want, tol = c.want()
+    c.seen, c.mask = seen, with_it
+    for b in range(2):
+        if int8:
+            c.k[b, at[b]] = c.tk[b, 0] = 0
+            c.k[b, at[b], :, 5] = c.tk[b, 0, :, 5] = -100
+            c.ks[b, at[b]] = c.tks[b, 0] = np.inf
+        else:
+            c.k[b, at[b], :, 5] = c.tk[b, 0, :, 5] = -np.inf
+    got = c.run(torch).cpu().numpy()
+    assert np.array_equal(lo, c.lo) and np.array_equal(hi, c.hi)
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / np.maximum(tol, 1e-30)).max())
+    # a NaN among the keys a row sees is the row's answer
+    if not int8:
+        c.k[:, :, :, 5] = np.nan
+        assert np.all(np.isnan(c.run(torch).cpu().numpy()))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_keys_at_the_top_of_the_range(cuda, int8):
+    """Keys and scales near the largest float under queries small enough for
+    finite scores."""
+    torch = cuda
+    for T in (1, 2, 9):
+        c = Tree(2, T, 12, 2, 48, 64, 90, 80, int8, seed=T)
+        c.q = np.clip(c.q, -4, 4) * np.float32(2.0 ** -122)
+        if int8:
+            for s in (c.ks, c.tks):
+                s *= np.float32(2.0 ** 121)
+        else:
+            c.k, c.tk = (np.clip(a, -4, 4) * np.float32(2.0 ** 122) for a in (c.k, c.tk))
+            c.k[:, ::7, :, 3] = np.float32(3.4028234663852886e38)
+            c.tk[:, :, :, 3] = -np.float32(3.4028234663852886e38)
+        c.check(torch)
