@@ -286,8 +286,8 @@ cudaError_t launch_logits_adjust(const float* x, int ldx, int rows, int vocab, f
   auto kern = bias_ids ? logits_kernel<true> : logits_kernel<false>;
   cudaError_t e = allow_smem((const void*)kern, smem, true);
   if (e != cudaSuccess) return e;
-  for (int r0 = 0; r0 < rows; r0 += 65535) {  // grid limit of the row axis
-    const int n = rows - r0 < 65535 ? rows - r0 : 65535;
+  for (long r0 = 0; r0 < rows; r0 += 65535) {  // grid limit of the row axis
+    const int n = (int)(rows - r0 < 65535 ? rows - r0 : 65535);
     LogitArgs B = A;
     B.x += (size_t)r0 * ldx;
     B.y += (size_t)r0 * ldy;

@@ -226,3 +226,26 @@ def test_keys_at_the_top_of_the_range(cuda, int8):
             c.k[:, ::7, :, 3] = np.float32(3.4028234663852886e38)
             c.tk[:, :, :, 3] = -np.float32(3.4028234663852886e38)
         c.check(torch)
+
+
+# ------------------------------------------------------------------ the largest counts
+MOST = 2 ** 31 - 1
+
+
+def _pieces(n, step=1 << 27):
+    return [slice(i, min(n, i + step)) for i in range(0, n, step)]
+
+
+def test_logits_of_the_largest_row_count(cuda):
+    """2^31 - 1 rows of one logit, in place, each with its pick."""
+    torch = cuda
+    x = torch.empty(MOST, device="cuda")
+    for s in _pieces(MOST):
+        x[s] = (torch.arange(s.start, s.stop, device="cuda") % 1009).float()
+    picks = torch.full((MOST,), -1, dtype=torch.int32, device="cuda")
+    nb.logits_adjust(ptr(x), 1, MOST, 1, ptr(x), 1, picks_ptr=ptr(picks))
+    for s in _pieces(MOST):
+        assert torch.equal(x[s], (torch.arange(s.start, s.stop, device="cuda") % 1009).float())
+        assert not picks[s].any()
+    del x, picks
+    torch.cuda.empty_cache()
