@@ -294,7 +294,7 @@ bool vec_ok(const void* p, int align) { return ((uintptr_t)p) % align == 0; }
 // 64: 31.1. f32 rows, 16384 written and read: 4: 31, 8: 21, 16: 18.6, 32: 16.3.
 static int kv_block_rows(int M, int pieces) {
   int rows = std::max(1, std::min(KV_ROWS, KV_THREADS * KV_FLIGHT / std::max(1, pieces)));
-  while (rows > 1 && (M + rows - 1) / rows < 148) rows /= 2;
+  while (rows > 1 && (M - 1) / rows + 1 < 148) rows /= 2;
   return rows;
 }
 
@@ -303,7 +303,7 @@ static cudaError_t launch_kv_rows(const KvRing& R, const int* sess, const int* p
                                   int ldv, cudaStream_t st) {
   const int nk = k ? R.kvh * R.qk / E : 0, nv = v ? R.kvh * R.vh / E : 0;
   const int rows = kv_block_rows(M, nk + nv);
-  kv_rows_kernel<INT8, E, WRITE><<<(M + rows - 1) / rows, KV_THREADS, 0, st>>>(
+  kv_rows_kernel<INT8, E, WRITE><<<(M - 1) / rows + 1, KV_THREADS, 0, st>>>(
       R, sess, pos, M, k, ldk, v, ldv, rows, FastDiv(nk + nv), FastDiv(std::max(1, R.qk / E)),
       FastDiv(std::max(1, R.vh / E)), nk);
   return cudaGetLastError();
@@ -344,8 +344,8 @@ cudaError_t launch_kv_append(const float* k, int ldk, const float* v, int ldv, c
   // 26.5, 8: 22.3, 16 (the rule): 19.3, 32: 20.7, 64: 22.7; the write alone 11.2.
   const int big = std::max(qk, vh), L = big <= 64 ? 16 : 32;
   int rows = std::max(1, std::min(KV_ROWS, (big > 128 ? 2 : KV_VECS) * (KV_THREADS / L) / (2 * kvh)));
-  while (rows > 1 && (M + rows - 1) / rows < 148) rows /= 2;
-  const int blocks = (M + rows - 1) / rows;
+  while (rows > 1 && (M - 1) / rows + 1 < 148) rows /= 2;
+  const int blocks = (M - 1) / rows + 1;
 #define NB_GO(V, L, S) \
   kv_append_i8_kernel<V, L, S>                \
       <<<blocks, KV_THREADS, 0, st>>>(k, ldk, v, ldv, sess, pos, M, R, rows, FastDiv(2 * kvh))

@@ -148,7 +148,7 @@ cudaError_t launch_rope(const float* x, int ldx, float* y, int ldy, const int* p
   int tok = 1;
   while (tok < 8 && (long)M > 592L * tok && items * tok < 1024) tok *= 2;
   const size_t smem = (size_t)tok * (rot + 1) * sizeof(float);
-  const dim3 grid((M + tok - 1) / tok);
+  const dim3 grid((M - 1) / tok + 1);
   const FastDiv ph(nhead), pt((uint32_t)items);
 #define NB_ROPE(V, I) \
   rope_kernel<V, I><<<grid, 256, smem, st>>>(x, ldx, y, ldy, pos, M, dim, rot, tok, ph, pt, F)

@@ -236,6 +236,51 @@ def _pieces(n, step=1 << 27):
     return [slice(i, min(n, i + step)) for i in range(0, n, step)]
 
 
+def test_rope_of_the_largest_row_count(cuda):
+    """2^31 - 1 rows in one call: every row as in calls of some of them."""
+    torch = cuda
+    x = torch.empty(MOST, 2, device="cuda")
+    pos = torch.empty(MOST, dtype=torch.int32, device="cuda")
+    for s in _pieces(MOST):
+        i = torch.arange(s.start, s.stop, device="cuda")
+        x[s, 0], x[s, 1], pos[s] = (i % 1009).float(), (i % 997).float(), (i % 65537).int()
+    nb.rope(ptr(x), 2, ptr(x), 2, ptr(pos), MOST, 1, 2)
+    torch.cuda.synchronize()
+    for s in _pieces(MOST):
+        i = torch.arange(s.start, s.stop, device="cuda")
+        y = torch.stack([(i % 1009).float(), (i % 997).float()], 1)
+        nb.rope(ptr(y), 2, ptr(y), 2, ptr(pos[s]), s.stop - s.start, 1, 2)
+        assert torch.equal(y, x[s])
+    del x, pos, i, y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_append_and_read_of_the_largest_row_count(cuda, int8):
+    """2^31 - 1 rows into a ring of as many places, and back."""
+    torch = cuda
+    src, pos = torch.empty(MOST, device="cuda"), torch.empty(MOST, dtype=torch.int32, device="cuda")
+    for s in _pieces(MOST):
+        i = torch.arange(s.start, s.stop, device="cuda")
+        src[s], pos[s] = (i % 1009 + 1).float(), (MOST - 1 - i).int()
+    sess = torch.zeros(MOST, dtype=torch.int32, device="cuda")
+    ring = [torch.empty(MOST, dtype=torch.int8 if int8 else torch.float32, device="cuda") for _ in range(2)]
+    sc = [torch.empty(MOST, device="cuda") if int8 else None for _ in range(2)]
+    nb.kv_append(ptr(src), 1, ptr(src), 1, ptr(sess), ptr(pos), MOST, int8, 1, MOST, 1, 1, 1, ptr(ring[0]),
+                 ptr(ring[1]), ptr(sc[0]), ptr(sc[1]))
+    back = torch.zeros(MOST, device="cuda")
+    for values in (False, True):
+        back.zero_()
+        nb.kv_read(ptr(ring[0]), ptr(ring[1]), ptr(sc[0]), ptr(sc[1]), int8, 1, MOST, 1, 1, 1, ptr(sess), ptr(pos),
+                   MOST, None if values else ptr(back), 1, ptr(back) if values else None, 1)
+        for s in _pieces(MOST):
+            # int8: the scale is one value's 127th, rounded, and 127 times that rounded again
+            want = src[s] / torch.full_like(src[s], 127.0) * 127.0 if int8 else src[s]
+            assert torch.equal(back[s], want)
+    del src, pos, sess, ring, sc, back, want, i
+    torch.cuda.empty_cache()
+
+
 def test_logits_of_the_largest_row_count(cuda):
     """2^31 - 1 rows of one logit, in place, each with its pick."""
     torch = cuda
