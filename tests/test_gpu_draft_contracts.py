@@ -294,3 +294,42 @@ def test_logits_of_the_largest_row_count(cuda):
         assert not picks[s].any()
     del x, picks
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ long sums
+@pytest.mark.parametrize("shape", [(1, 4, 1, 128, 128, 5651), (2, 4, 1, 32, 32, 6007), (1, 12, 2, 48, 64, 9001),
+                                   (9, 4, 1, 128, 128, 5651), (4, 12, 2, 48, 64, 9001), (16, 12, 2, 64, 64, 7013)])
+@pytest.mark.parametrize("int8", [False, True])
+def test_long_sums_stay_within_a_quarter_of_the_32_bit_forms_error(cuda, int8, shape):
+    """Against 64 bits, relative to the whole output: at most 1.25 times the error
+    of the same attention in plain 32-bit products and sums, or 1.5 * 2^-22 where
+    that is more. The floor is the kernels' own arithmetic, as independent errors
+    of the weights: an exponential's 2^-22 (rms 1.4e-7), the rounding of its argument
+    of up to 8 (2^-22 ln 2, rms 1.0e-7), the 22 bits of query, key and weight (below
+    0.7e-7 each), the f32 additions of a warp's blocks (at most 90 here, 1.6e-7 as a
+    random walk): together 2.7e-7. Sums left to accumulators that truncate were
+    at 8.4e-7 over 5651 positions."""
+    torch = cuda
+    T, heads, kvh, qk, vh, ctx = shape
+    c = Tree(1, T, heads, kvh, qk, vh, ctx, ctx, int8, seed=ctx)
+    c.lo[:] = 0
+    c.hi[:] = ctx - 1
+    c.mask[:] = 0
+    got = c.run(torch)[0].double()
+    k, v = (torch.from_numpy(a[0].astype(np.float64)).cuda() for a in (c.k, c.v))
+    if int8:
+        k, v = (a * torch.from_numpy(s[0].astype(np.float64)).cuda()[..., None] for a, s in ((k, c.ks), (v, c.vs)))
+    q = torch.from_numpy(c.q[0, :, : heads * qk].reshape(T, heads, qk)).cuda().double()
+
+    def attend(dt):
+        kk, vv = (a.to(dt).repeat_interleave(heads // kvh, 1).transpose(0, 1) for a in (k, v))
+        s = q.to(dt).transpose(0, 1) @ kk.transpose(1, 2) / qk ** 0.5
+        w = torch.exp(s - s.amax(-1, keepdim=True))
+        return (w @ vv / w.sum(-1, keepdim=True)).transpose(0, 1).double()
+
+    old = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    want, plain = attend(torch.float64), attend(torch.float32)
+    torch.backends.cuda.matmul.allow_tf32 = old
+    mine, theirs = (float((x - want).norm() / want.norm()) for x in (got, plain))
+    assert mine <= max(1.25 * theirs, 1.5 * 2.0 ** -22), (mine, theirs)
