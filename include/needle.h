@@ -349,7 +349,10 @@ int nd_kv_read(const void *kc, const void *vc, const float *ks, const float *vs,
  * NULL: the ring only. out [B][T][heads][vh]; a node that sees nothing gets
  * zeros, and what a node does not see never reaches its output, whatever it
  * holds. heads / kv_heads may be any number; qk and vh multiples of 4 up to 128;
- * T up to 4096. T = 1 is one decode step. Scores are scaled by 1 / sqrt(qk).
+ * T up to 4096; rings and draft 4-byte aligned. T = 1 is one decode step.
+ * Queries are taken as they are: to verify what the reference decodes from an
+ * int8 cache, pass them fake-quantised, as for nd_attend_step (nd_kv_quant, then
+ * nd_kv_read of its codes). Scores are scaled by 1 / sqrt(qk).
  * out must not overlap an input. Partial results of long rings use
  * stream-ordered scratch. Rows left NaN by a wait that gave up are told by
  * nd_take_wait_error below. */

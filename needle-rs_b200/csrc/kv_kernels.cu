@@ -1,8 +1,9 @@
-// Standalone writes to and reads from the KV rings of nd_attend_step's layout
-// (k [sessions][slots][kv_heads][qk], v [..][vh], scales [..][kv_heads]):
+// Standalone writes to and reads from KV rings of nd_attend_step's layout (k
+// [sessions][slots][kv_heads][qk], v [..][vh], scales [..][kv_heads]):
 // nd_kv_append quantises as it writes, nd_kv_read gives back the values. The
-// quantiser is the engine's own rule (kv_quant_codes, common.cuh), so a ring
-// filled here equals the engine's bit for bit.
+// quantiser is the engine's rule (kv_quant_codes, common.cuh), so codes and scales
+// equal the engine's bit for bit; the rings do not, as a session's own are
+// head-major and hold value codes offset by 128.
 #include <algorithm>
 
 #include "fastdiv.hpp"

@@ -6,7 +6,7 @@ where nothing else stands beside the comparison.
 """
 import numpy as np
 import pytest
-from conftest import nb
+from conftest import nb, orc
 from test_gpu_draft import ROPE_TOL, Tree, dev, ptr, quant_ref, rope_ref
 
 pytestmark = pytest.mark.gpu
@@ -333,3 +333,41 @@ def test_long_sums_stay_within_a_quarter_of_the_32_bit_forms_error(cuda, int8, s
     torch.backends.cuda.matmul.allow_tf32 = old
     mine, theirs = (float((x - want).norm() / want.norm()) for x in (got, plain))
     assert mine <= max(1.25 * theirs, 1.5 * 2.0 ** -22), (mine, theirs)
+
+
+# ------------------------------------------------------------------ a layer as a server runs it
+def fake_quantised(torch, q, rows, heads, qk):
+    """Queries [rows][heads * qk] through the int8 codes and back, in place: the
+    scales of nd_kv_quant, the values of nd_kv_read."""
+    codes = torch.empty(rows, heads, qk, dtype=torch.int8, device="cuda")
+    scales = torch.empty(rows, heads, device="cuda")
+    zero = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    nb.kv_quant(ptr(q), rows * heads, qk, ptr(codes), ptr(scales))
+    nb.kv_read(ptr(codes), None, ptr(scales), None, True, rows, 1, heads, qk, qk, None, ptr(zero), rows, ptr(q),
+               heads * qk, None, 0)
+
+
+def test_an_int8_draft_is_verified_as_the_reference_decodes(cuda):
+    """Queries fake-quantised on the device equal the reference's to the bit, and
+    each node of a chain equals the reference's decode step (fake-quantised query,
+    the earlier nodes in the ring)."""
+    torch = cuda
+    B, T, H, kvh, qk, vh, slots = 3, 6, 12, 2, 48, 64, 96
+    c = Tree(B, T, H, kvh, qk, vh, slots, 70, True, seed=3, mask="chain")
+    q = dev(torch, c.q)
+    fake_quantised(torch, q, B * T, H, qk)
+    got_q = q.cpu().numpy()
+    want_q = np.stack([orc.fake_quant(v) for v in c.q.reshape(-1, qk)]).reshape(c.q.shape)
+    assert np.array_equal(got_q, want_q) and not np.array_equal(got_q, c.q)
+    c.q = got_q
+    got = c.check(torch)
+    _, tol = c.want()
+    for b in range(B):
+        k, v, ks, vs = (a[b].copy() for a in (c.k, c.v, c.ks, c.vs))
+        for t in range(T):
+            at = int(c.hi[b, t]) + 1 + t
+            k[at % slots], v[at % slots], ks[at % slots], vs[at % slots] = c.tk[b, t], c.tv[b, t], c.tks[b, t], c.tvs[b, t]
+            want = orc.attend_step(got_q[b, t], slots, int(c.lo[b, t]), at, H, kvh, qk, vh, kq=k.ravel(),
+                                   ks=ks.ravel(), vq=v.ravel(), vs=vs.ravel())
+            # the oracle sums in f32 itself: within its own rounding, the bound again
+            assert np.all(np.abs(got[b, t] - np.asarray(want).reshape(H, vh)) <= 2 * tol[b, t])
