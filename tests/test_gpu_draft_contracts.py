@@ -6,8 +6,9 @@ where nothing else stands beside the comparison.
 """
 import numpy as np
 import pytest
-from conftest import nb, orc
-from test_gpu_draft import ROPE_TOL, Tree, dev, ptr, quant_ref, rope_ref
+from conftest import cact_pack, nb, orc
+from test_gpu_draft import LOGIT_TOL, ROPE_TOL, Tree, dev, logits_ref, ptr, quant_ref, rope_ref
+from test_gpu_kernels import close, make_weight
 
 pytestmark = pytest.mark.gpu
 
@@ -371,3 +372,101 @@ def test_an_int8_draft_is_verified_as_the_reference_decodes(cuda):
                                    ks=ks.ravel(), vq=v.ravel(), vs=vs.ravel())
             # the oracle sums in f32 itself: within its own rounding, the bound again
             assert np.all(np.abs(got[b, t] - np.asarray(want).reshape(H, vh)) <= 2 * tol[b, t])
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_drafted_layer_from_projection_to_picks(cuda, int8):
+    """Hidden states to picks of a tree's nodes as one run of calls: project q | k
+    | v, rotate, append to the draft, attend, project to logits, correct and pick,
+    append the accepted path. Every step's output is held against its reference
+    on what the step before it left."""
+    torch = cuda
+    B, H, kvh, qk, vh, slots, V, d = 3, 12, 2, 48, 64, 90, 812, 768
+    parents, path = [-1, 0, 0, 1, 3, 2, 4], [0, 1, 3, 4, 6]
+    T, N = len(parents), 3 * len(parents)
+    depth = [0] * T
+    for t, p in enumerate(parents):
+        depth[t] = depth[p] + 1 if p >= 0 else 0
+    rng = np.random.default_rng(8)
+    cb = cact_pack.random_codebook(np.random.default_rng(9))
+    levels = cact_pack.codebook_levels(cb, 2)
+    shapes = (H * qk, kvh * qk, kvh * vh)
+    mats = [make_weight(torch, o, d, 2, 50 + i, cb) for i, o in enumerate(shapes)]
+    head = make_weight(torch, V, d, 2, 60, cb)
+    ld = sum(shapes)
+    c = Tree(B, T, H, kvh, qk, vh, slots, 80, int8, seed=12)
+    c.mask = np.repeat(nb.tree_mask(parents)[None], B, 0)
+    ring = [dev(torch, a) for a in (c.k, c.v, c.ks, c.vs)]
+    pos = np.array([[c.hi[b, 0] + 1 + depth[t] for t in range(T)] for b in range(B)], np.int32).ravel()
+    sess, node = np.repeat(np.arange(B), T).astype(np.int32), np.tile(np.arange(T), B).astype(np.int32)
+    kept = np.where(np.isin(node, path), pos, -1).astype(np.int32)
+    posd, sessd, noded, keptd, lo, hi, mask = (dev(torch, a) for a in (pos, sess, node, kept, c.lo, c.hi, c.mask.view(np.int32)))
+    hist = rng.integers(0, V, 40 * N).astype(np.int32)
+    off = (np.arange(N + 1) * 40).astype(np.int32)
+    gen = off[:-1] + 20
+    rep, pres, freq = (rng.uniform(a, b, N).astype(np.float32) for a, b in ((1.0, 1.5), (0.0, 0.5), (0.0, 0.3)))
+    keep = rng.random((N, V)) < 0.5
+    hd, od, gd, rd, pd, fd, bits = (dev(torch, a) for a in (hist, off, gen, rep, pres, freq, nb.pack_mask(keep).view(np.int32)))
+    dt = torch.int8 if int8 else torch.float32
+    draft = [torch.zeros(B, T, kvh, w, dtype=dt, device="cuda") for w in (qk, vh)]
+    draft += [torch.zeros(B, T, kvh, device="cuda") if int8 else None for _ in range(2)]
+    x = (rng.normal(size=(N, d)) * 3).astype(np.float32)
+    xd, xh, oh = dev(torch, x), torch.zeros(N, d, device="cuda"), torch.zeros(N, d, device="cuda")
+    rows, q = torch.zeros(N, ld, device="cuda"), torch.zeros(N, H * qk, device="cuda")
+    out, logits = torch.zeros(B, T, H, vh, device="cuda"), torch.zeros(N, V, device="cuda")
+    picks = torch.zeros(N, dtype=torch.int32, device="cuda")
+    at_k, at_v = 4 * H * qk, 4 * (H + kvh) * qk
+
+    # ---- the run of calls
+    nb.cq_prepare(ptr(xd), N, d, ptr(xh), d)
+    nb.cq_project_grouped([(m[1], m[2], o) for m, o in zip(mats, shapes)], d, 2, levels, ptr(xh), d, N, ptr(rows), ld)
+    projected = rows.clone()
+    nb.rope(ptr(rows), ld, ptr(q), H * qk, ptr(posd), N, H, qk)
+    nb.rope(ptr(rows) + at_k, ld, ptr(rows) + at_k, ld, ptr(posd), N, kvh, qk)
+    rotated = q.clone()
+    if int8:
+        fake_quantised(torch, q, N, H, qk)
+    nb.kv_append(ptr(rows) + at_k, ld, ptr(rows) + at_v, ld, ptr(sessd), ptr(noded), N, int8, B, T, kvh, qk, vh,
+                 *[ptr(a) for a in draft])
+    nb.attend_tree(ptr(q), H * qk, *[ptr(a) for a in ring], int8, slots, ptr(lo), ptr(hi), *[ptr(a) for a in draft],
+                   ptr(mask), B, T, H, kvh, qk, vh, ptr(out))
+    nb.cq_prepare(ptr(out), N, d, ptr(oh), d)
+    nb.cq_project(head[1], head[2], V, d, 2, levels, ptr(oh), d, N, ptr(logits), V)
+    plain = logits.clone()
+    nb.logits_adjust(ptr(logits), V, N, V, ptr(logits), V, ptr(hd), ptr(od), ptr(gd), ptr(rd), ptr(pd), ptr(fd),
+                     mask_ptr=ptr(bits), mask_ld=(V + 31) // 32, masked=-1e9, picks_ptr=ptr(picks))
+    nb.kv_append(ptr(rows) + at_k, ld, ptr(rows) + at_v, ld, ptr(sessd), ptr(keptd), N, int8, B, slots, kvh, qk, vh,
+                 *[ptr(a) for a in ring])
+
+    # ---- each step against its reference
+    xh_want = np.stack([mats[0][3].prepare(r) for r in x])
+    assert close(projected.cpu().numpy(), np.concatenate([m[3].matmul_prepared(xh_want) for m in mats], 1))
+    proj = projected.cpu().numpy()
+    for got, a, n in ((rotated, 0, H), (rows[:, H * qk: (H + kvh) * qk], H * qk, kvh)):
+        want, size = rope_ref(proj[:, a: a + n * qk], pos, n, qk, qk, 10000.0, False, None, False)
+        assert np.all(np.abs(got.cpu().numpy() - want) <= ROPE_TOL * size)
+    if int8:
+        want = np.stack([orc.fake_quant(v) for v in rotated.cpu().numpy().reshape(-1, qk)])
+        assert np.array_equal(q.cpu().numpy().reshape(-1, qk), want)
+    r = rows.cpu().numpy()
+    k, v = r[:, H * qk: (H + kvh) * qk].reshape(N, kvh, qk), r[:, (H + kvh) * qk:].reshape(N, kvh, vh)
+    (ck, sk), (cv, sv) = (quant_ref(k), quant_ref(v)) if int8 else ((k, None), (v, None))
+    for a, w in zip(draft, (ck, cv, sk, sv)):
+        assert a is None or np.array_equal(a.cpu().numpy().reshape(w.shape), w)
+    c.q, c.ldq = q.cpu().numpy().reshape(B, T, H * qk), H * qk
+    c.tk, c.tv, c.tks, c.tvs = (None if a is None else a.cpu().numpy() for a in draft)
+    want, tol = c.want()
+    assert np.all(np.abs(out.cpu().numpy() - want) <= tol)
+    o = out.cpu().numpy().reshape(N, d)
+    assert close(plain.cpu().numpy(), head[3].matmul_prepared(np.stack([head[3].prepare(a) for a in o])))
+    got = logits.cpu().numpy()
+    want, size = logits_ref(plain.cpu().numpy(), hist, off, gen, rep, pres, freq, None, None, None, keep, -1e9)
+    assert np.all(np.abs(got - want) <= LOGIT_TOL * size)
+    assert np.array_equal(picks.cpu().numpy(), got.argmax(1))
+    final = [None if a is None else a.copy() for a in (c.k, c.v, c.ks, c.vs)]
+    for i in np.flatnonzero(kept >= 0):
+        for a, w in zip(final, (ck, cv, sk, sv)):
+            if a is not None:
+                a[sess[i], kept[i] % slots] = w[i]
+    for a, w in zip(ring, final):
+        assert a is None or np.array_equal(a.cpu().numpy(), w)
