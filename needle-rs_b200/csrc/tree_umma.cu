@@ -69,7 +69,7 @@ struct TreeUmma {
                        REG_SOFT = I8 ? (TPR == 1 ? 184 : 176) : VP == 64 ? 144 : 160,
                        REG_PROD = ((TPR + PWG) * REG_ALL - TPR * REG_SOFT) / PWG;
   static_assert(TPR * REG_SOFT + PWG * REG_PROD == (TPR + PWG) * REG_ALL && REG_PROD % 8 == 0 &&
-                    THREADS * CTAS * REG_ALL <= 65536,
+                    THREADS * CTAS * REG_ALL <= 65536 && REG_SOFT >= REG_ALL,
                 "register shares");
   static constexpr int TMEM = 2 * BN + VP <= 128 ? 128 : 256;  // columns: two of S (then P), O
   static constexpr size_t META = NST * (size_t)(BN * 8 + 16 + 16) + 128 * 4 + 512 + 2 * 2 * 128 * 4;
@@ -909,14 +909,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TMEM));
   }
-  // ---- rows to do again, a warp each
+  // ---- rows to do again, a warp each: the softmax warps, whose register share is
+  // no smaller than the launch's (the others gave theirs up, and code past the
+  // roles need not keep to what they have left)
   for (int wd = 0; wd < 4; ++wd) {
     uint32_t todo = slow[wd];
     int turn = 0;
     while (todo) {
       const int r2 = wd * 32 + __ffs(todo) - 1;
       todo &= todo - 1;
-      if (turn++ % (C::THREADS / 32) != warp) continue;
+      if (turn++ % (TPR * 4) != warp) continue;
       const int q2 = r0 + r2, n2 = A.by_rep.div(q2), h2 = kh * A.rep + q2 - n2 * A.rep;
       const size_t at2 = (size_t)b * A.T + n2;
       const int hh = A.hi[at2];

@@ -229,6 +229,20 @@ def test_keys_at_the_top_of_the_range(cuda, int8):
         c.check(torch)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("T,heads,kvh,qk,vh,slots", [(65, 4, 1, 48, 64, 300), (40, 8, 2, 64, 64, 90), (33, 8, 2, 128, 128, 200),
+                                                     (70, 2, 1, 128, 128, 4200), (150, 1, 1, 48, 64, 5000)])
+def test_every_row_done_again(cuda, int8, T, heads, kvh, qk, vh, slots):
+    """Keys above 2^96 under queries as small: no row of a tile can stay with split
+    operands, whole and partial results alike."""
+    torch = cuda
+    c = Tree(1, T, heads, kvh, qk, vh, slots, slots - 9, int8, seed=T)
+    c.q = c.q * np.float32(2.0 ** -110)
+    for n in ("ks", "tks") if int8 else ("k", "tk"):
+        setattr(c, n, getattr(c, n) * np.float32(2.0 ** 110))
+    c.check(torch)
+
+
 # ------------------------------------------------------------------ the largest counts
 MOST = 2 ** 31 - 1
 
