@@ -484,3 +484,132 @@ def test_a_drafted_layer_from_projection_to_picks(cuda, int8):
                 a[sess[i], kept[i] % slots] = w[i]
     for a, w in zip(ring, final):
         assert a is None or np.array_equal(a.cpu().numpy(), w)
+
+
+# ------------------------------------------------------------------ the ends of the documented ranges
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("shape", [
+    # B, T, heads, kv_heads, qk, vh, slots, ctx
+    (1, 3, 301, 1, 48, 64, 40, 33),      # hundreds of query heads a KV head
+    (2, 1, 512, 512, 16, 16, 30, 21),    # the most KV heads
+    (1, 2, 1024, 512, 4, 4, 20, 17),
+    (3, 5, 6, 2, 4, 4, 33, 30),          # the narrowest heads
+    (1, 40, 4, 2, 4, 128, 50, 41),
+    (2, 20, 2, 1, 128, 16, 7, 7),
+])
+def test_tree_attention_at_the_ends_of_its_ranges(cuda, int8, shape):
+    B, T, heads, kvh, qk, vh, slots, ctx = shape
+    Tree(B, T, heads, kvh, qk, vh, slots, ctx, int8, seed=sum(shape), extra=T % 3).check(cuda)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_the_most_nodes(cuda, int8):
+    """4096 nodes: 128 mask words a node, a chain and a tree; a few rows by 64 bits."""
+    torch = cuda
+    for mask in ("chain", "tree"):
+        c = Tree(1, 4096, 2, 1, 16, 16, 50, 41, int8, seed=6, mask=mask)
+        got = c.run(torch).cpu().numpy()
+        rows = sorted({0, 1, 31, 32, 63, 64, 127, 128, 2047, 2048, 4094, 4095})
+        seen = {t: c.seen(0, t) for t in rows}
+        q, c.T = c.q, 1                 # Tree.want of one node at a time
+        for t in rows:
+            c.q, c.seen = q[:, t: t + 1], lambda b, u, t=t: seen[t]
+            want, tol = c.want()
+            assert np.all(np.abs(got[:, t] - want[:, 0]) <= tol[:, 0]), (mask, t)
+        assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("T", [1, 3, 20])
+def test_a_ring_of_2_to_the_30_places(cuda, T):
+    """Windows at both ends of the largest ring, in one call and one row tile."""
+    torch = cuda
+    slots, d = 1 << 30, 16
+    k, v = (torch.zeros(slots, d, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.ones(slots, device="cuda") for _ in range(2))
+    near, far = slice(5, 105), slice(slots - 100, slots)
+    for s in (near, far):
+        v[s] = torch.randint(-127, 128, (100, d), dtype=torch.int8, device="cuda")
+    q = torch.zeros(T, d, device="cuda")
+    lo = torch.tensor([5 if t % 2 else slots - 100 for t in range(T)], dtype=torch.int32, device="cuda")
+    hi = lo + 99
+    if T > 2:  # across the ring's end: the last 100 places and the first 105
+        lo[2], hi[2] = slots - 100, slots + 104
+    out = torch.zeros(T, d, device="cuda")
+    nb.attend_tree(ptr(q), d, ptr(k), ptr(v), ptr(ks), ptr(vs), True, slots, ptr(lo), ptr(hi), None, None, None, None,
+                   None, 1, T, 1, 1, d, d, ptr(out))
+    want = [(v[near] if t % 2 else v[far]).double().mean(0) for t in range(T)]
+    if T > 2:
+        want[2] = torch.cat([v[far], v[:105]]).double().mean(0)
+    # weights of 1: sums of whole numbers below 2^24, one division
+    assert ((out.double() - torch.stack(want)).abs() <= 2.0 ** -20 * 127).all()
+    del k, v, ks, vs
+    torch.cuda.empty_cache()
+
+
+def test_append_of_the_most_heads(cuda):
+    torch = cuda
+    for int8 in (False, True):
+        M, kvh, qk, vh = 5, 512, 12, 256
+        x = np.random.default_rng(0).normal(size=(M, kvh * (qk + vh))).astype(np.float32)
+        xd = dev(torch, x)
+        pos = torch.arange(M, dtype=torch.int32, device="cuda") % 2
+        sess = torch.arange(M, dtype=torch.int32, device="cuda") // 2
+        dt = torch.int8 if int8 else torch.float32
+        ring = [torch.zeros(3, 2, kvh, w, dtype=dt, device="cuda") for w in (qk, vh)]
+        sc = [torch.zeros(3, 2, kvh, device="cuda") if int8 else None for _ in range(2)]
+        nb.kv_append(ptr(xd), x.shape[1], ptr(xd) + 4 * kvh * qk, x.shape[1], ptr(sess), ptr(pos), M, int8, 3, 2, kvh,
+                     qk, vh, ptr(ring[0]), ptr(ring[1]), ptr(sc[0]), ptr(sc[1]))
+        for a, s, part, w in ((ring[0], sc[0], x[:, : kvh * qk], qk), (ring[1], sc[1], x[:, kvh * qk:], vh)):
+            want = part.reshape(M, kvh, w)
+            if int8:
+                want, scales = quant_ref(want)
+                assert np.array_equal(s.cpu().numpy().reshape(6, kvh)[:M], scales)
+            assert np.array_equal(a.cpu().numpy().reshape(6, kvh, w)[:M], want)
+
+
+def test_logits_of_the_largest_vocabulary(cuda):
+    """2^30 ids: history, biases and mask at both ends, in place."""
+    torch = cuda
+    V = 1 << 30
+    x = torch.zeros(V, device="cuda")
+    x[V - 2], x[3], x[V // 2] = 9.0, 8.0, 8.5
+    mask = torch.full((V // 32,), -1, dtype=torch.int32, device="cuda")
+    mask[V // 64] = -2                                  # V / 2 forbidden
+    hist = torch.tensor([V - 2, V - 1, V - 2, -1], dtype=torch.int32, device="cuda")
+    ids = torch.tensor([V - 1, 0, V - 1], dtype=torch.int32, device="cuda")
+    vals = torch.tensor([2.0, 1.0, 4.0], device="cuda")
+    ends = [torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (4, 3)]
+    rep, pres, freq = (torch.tensor([a], device="cuda") for a in (2.0, 0.25, 0.5))
+    picks = torch.zeros(1, dtype=torch.int32, device="cuda")
+    nb.logits_adjust(ptr(x), V, 1, V, ptr(x), V, ptr(hist), ptr(ends[0]), None, ptr(rep), ptr(pres), ptr(freq), ptr(ids),
+                     ptr(vals), ptr(ends[1]), ptr(mask), V // 32, -1e9, ptr(picks))
+    at = [V - 2, V - 1, V // 2, 3, 0]
+    assert x[at].cpu().tolist() == [9.0 / 2 - 1.25, 6.0 - 0.75, -1e9, 8.0, 1.0] and int(picks[0]) == 3
+    x[at] = 0.0
+    assert not x.any()
+    del x, mask
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_joined_decode_step_in_two_graphs(cuda, int8):
+    """One token over a long ring (partial results in scratch, a second kernel):
+    two graphs replayed on two streams at once, and again."""
+    torch = cuda
+    sets = []
+    for seed in (1, 2):
+        c = Tree(1, 1, 6, 1, 48, 64, 9000, 8900, int8, seed=seed, drafted=False)
+        want = torch.from_numpy(c.check(torch)).cuda()
+        out, stream, g = torch.zeros_like(want), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            c.call(c.keep, out, stream.cuda_stream)
+        sets.append((c, want, out, stream, g))
+    for _ in range(5):
+        for _, _, out, _, _ in sets:
+            out.fill_(3)
+        torch.cuda.synchronize()
+        for _, _, _, stream, g in sets:
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for _, want, out, _, _ in sets)
