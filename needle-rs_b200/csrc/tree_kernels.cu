@@ -150,34 +150,55 @@ __device__ __forceinline__ void tree_copy(char* buf, const char* k, const char* 
   }
 }
 
-// Row rr of KV head kh again over one warp's blocks of PB positions (blk0, blk0 +
-// TREE_WARPS .. below blk1; the ring's blocks first) in plain f32, into `row`:
-// outputs, and its max and sum at [at], [at + 1].
-template <bool I8>
-__device__ __noinline__ void tree_again(const TreeArgs& A, int b, int kh, int rr, int base, int n_ring, int PB,
-                                        int ring_blocks, int blk0, int blk1, float* row, int at) {
+// A warp's rows again, over its own blocks of PB positions and in plain f32: those
+// whose sum is no number, or all of them, of the TILE rows of `mine` (row stride
+// PW: outputs, then max and sum at AT). Everything is worked out afresh, so that
+// the kernel keeps no register for it (with the ranges handed over the 128-wide
+// forms were 5 to 7 % slower; so, f32 ones are 3 %: 32 x 1043 with 6 rows 218 -> 225
+// us, int8 50.1 -> 49.9).
+template <bool I8, int TILE, int PB, int PW, int AT>
+__device__ __noinline__ void tree_again(const TreeArgs& A, float* mine, bool all) {
+  const int b = blockIdx.y, wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int z = blockIdx.x % A.nsplit, kh = blockIdx.x / A.nsplit % A.kvh, tile = blockIdx.x / A.nsplit / A.kvh;
+  const int R = A.T * A.rep, r0 = tile * TILE, rows = min(TILE, R - r0);
+  int first = 0x7fffffff, last = -1;
+  for (int n = A.by_rep.div(r0) + lane; n <= A.by_rep.div(r0 + rows - 1); n += 32) {
+    const int h = A.hi[(size_t)b * A.T + n];
+    int l = max(A.lo[(size_t)b * A.T + n], 0);
+    if (h >= 0) l = max(l, h - A.slots + 1);
+    if (l <= h) first = min(first, l), last = max(last, h);
+  }
+  first = __reduce_min_sync(0xffffffffu, first), last = __reduce_max_sync(0xffffffffu, last);
+  const int base = last >= 0 ? first : 0, n_ring = last >= 0 ? (int)min((long)last - base + 1, (long)A.slots) : 0;
+  const int ring_blocks = (n_ring + PB - 1) / PB, blocks = ring_blocks + (A.drafted + PB - 1) / PB;
+  const int blk0 = (int)((long)blocks * z / A.nsplit) + wid, blk1 = (int)((long)blocks * (z + 1) / A.nsplit);
   TreePlace P;
   P.ring = (size_t)b * A.slots * A.kvh + kh, P.draft = (size_t)b * A.T * A.kvh + kh;
   P.drafted = A.drafted, P.slot0 = base % A.slots, P.slots = A.slots, P.kvh = A.kvh, P.total = A.drafted + n_ring;
-  const int node = A.by_rep.div(rr), head = kh * A.rep + rr - node * A.rep, lane = threadIdx.x & 31;
-  const size_t node_at = (size_t)b * A.T + node;
-  const int h = A.hi[node_at];
-  int l = max(A.lo[node_at], 0);
-  if (h >= 0) l = max(l, h - A.slots + 1);
-  const int cnt = l <= h ? h - l + 1 : 0, start = cnt ? (int)((long)(l - base) % A.slots) : 0;
-  const float* q = A.q + node_at * A.ldq + (size_t)head * A.qk;
-  bool none = false;
-  for (int i = lane; i < A.qk; i += 32) none |= q[i] != q[i];
-  if (__any_sync(0xffffffffu, none)) return;  // a NaN in the query: NaN it stays
-  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int blk = blk0; blk < blk1; blk += TREE_WARPS) {
-    const int v0 = blk < ring_blocks ? P.drafted + blk * PB : (blk - ring_blocks) * PB;
-    tree_slow_row<I8>(A, P, node_at, node, head, start, cnt, n_ring, v0,
-                      min(v0 + PB, blk < ring_blocks ? P.total : P.drafted), &m, &sum, o);
+  for (int r = 0; r < rows; ++r) {
+    float* row = mine + (size_t)r * PW;
+    if (!all && row[AT + 1] <= 3.4028234e38f) continue;
+    const int rr = r0 + r, node = A.by_rep.div(rr), head = kh * A.rep + rr - node * A.rep;
+    const size_t node_at = (size_t)b * A.T + node;
+    const float* q = A.q + node_at * A.ldq + (size_t)head * A.qk;
+    bool none = false;
+    for (int i = lane; i < A.qk; i += 32) none |= q[i] != q[i];
+    if (__any_sync(0xffffffffu, none)) continue;  // a NaN in the query: NaN it stays
+    const int h = A.hi[node_at];
+    int l = max(A.lo[node_at], 0);
+    if (h >= 0) l = max(l, h - A.slots + 1);
+    const int cnt = l <= h ? h - l + 1 : 0, start = cnt ? (int)((long)(l - base) % A.slots) : 0;
+    float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int blk = blk0; blk < blk1; blk += TREE_WARPS) {
+      const int v0 = blk < ring_blocks ? P.drafted + blk * PB : (blk - ring_blocks) * PB;
+      tree_slow_row<I8>(A, P, node_at, node, head, start, cnt, n_ring, v0,
+                        min(v0 + PB, blk < ring_blocks ? P.total : P.drafted), &m, &sum, o);
+    }
+    __syncwarp();  // the row's sum has been read
+    for (int j = 0; j < 4; ++j)
+      if (lane + 32 * j < A.vh) row[lane + 32 * j] = o[j];
+    if (lane == 0) row[AT] = m, row[AT + 1] = sum;
   }
-  for (int j = 0; j < 4; ++j)
-    if (lane + 32 * j < A.vh) row[lane + 32 * j] = o[j];
-  if (lane == 0) row[at] = m, row[at + 1] = sum;
 }
 
 // Grid (row tiles * kvh * nsplit, B), four warps: each holds the same MT * 16
@@ -192,7 +213,7 @@ __global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const __grid_
   constexpr int PB = TT::PB, NT = PB / 8;        // 8-position score tiles of a block
   constexpr int KC = QKP / 16, VN = VHP / 8;     // 16-dim chunks of a key, 8-dim tiles of an output
   extern __shared__ __align__(16) char smem[];
-  __shared__ int range[4];  // lowest and highest seen position, longest unseen head, shortest seen end
+  __shared__ int range[3];  // lowest and highest seen position; int8: whether a score may have passed the range
   const int b = blockIdx.y;
   int bx = blockIdx.x;
   const int z = bx % A.nsplit;
@@ -203,7 +224,7 @@ __global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const __grid_
   const int n0 = A.by_rep.div(r0), n1 = A.by_rep.div(r0 + rows - 1);  // first and last node of the tile
 
   // Ring range of the tile. Each node's lo is held within one turn of the ring.
-  if (tid == 0) range[0] = 0x7fffffff, range[1] = -1;
+  if (tid == 0) range[0] = 0x7fffffff, range[1] = -1, range[2] = 0;
   __syncthreads();
   for (int n = n0 + tid; n <= n1; n += TREE_THREADS) {
     const int h = A.hi[(size_t)b * A.T + n];
@@ -349,7 +370,6 @@ __global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const __grid_
   float o[MT][VN][4], mx[2 * MT], sum[2 * MT];
   int vexp, vlow;         // int8: outputs are held times 2^(140 - vexp); least exponent of a value scale
   bool careful = false;   // a second run over the blocks, see below
-  bool far = false;       // int8: a score may have passed the range
 again:
   vexp = 14, vlow = 255;
 #pragma unroll
@@ -510,7 +530,7 @@ again:
     float grow = 1.f;
     float2 v2[NT];
     if (I8) {
-      far |= fabsf(sc[lane]) > 0x1p96f;  // times a product of up to 2^28
+      if (fabsf(sc[lane]) > 0x1p96f) range[2] = 1;  // times a product of up to 2^28
       const uint32_t a = __float_as_uint(fabsf(sc[PB + lane]));
       const uint32_t top = __reduce_max_sync(0xffffffffu, a);
       vlow = min(vlow, (int)(__reduce_min_sync(0xffffffffu, a ? a : 0x7f800000u) >> 23));
@@ -665,7 +685,7 @@ again:
 #pragma unroll
       for (int n = 0; n < VN; ++n) o[m][n][0] *= f, o[m][n][1] *= f, o[m][n][2] *= f, o[m][n][3] *= f;
   }
-  bool lost = far;
+  bool lost = false;
 #pragma unroll
   for (int i = 0; i < 2 * MT; ++i) {
     sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
@@ -689,15 +709,10 @@ again:
   // remainder is NaN, but its score may be -inf and weigh nothing) are done again,
   // and so is every row where a score may have passed the range before the query's
   // power of two is taken back.
-  if (__any_sync(0xffffffffu, lost)) {
+  const bool far = I8 && *(volatile int*)(range + 2);
+  if (__builtin_expect(__any_sync(0xffffffffu, lost || far), 0)) {
     __syncwarp();
-    far = __any_sync(0xffffffffu, far);
-#pragma unroll 1
-    for (int r = 0; r < rows; ++r) {
-      float* row = P + ((size_t)wid * MT * 16 + r) * PW;
-      if (far || !(row[VHP + 1] <= 3.4028234e38f))
-        tree_again<I8>(A, b, kh, r0 + r, base, n_ring, PB, ring_blocks, blk0, blk1, row, VHP);
-    }
+    tree_again<I8, MT * 16, PB, PW, VHP>(A, P + (size_t)wid * MT * 16 * PW, far);
   }
   __syncthreads();
   // Splits of a cluster: each block leaves its rows (outputs, max, sum) in warp

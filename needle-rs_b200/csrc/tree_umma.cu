@@ -156,6 +156,15 @@ __device__ __forceinline__ void widen(uint32_t u, uint32_t* a, uint32_t* b) {
   *a = *reinterpret_cast<uint32_t*>(&x);
   *b = *reinterpret_cast<uint32_t*>(&y);
 }
+// tree_slow_row out of line: inlined, it cost the roles registers (48 nodes f32 65.8
+// -> 72 us).
+template <bool I8>
+__device__ __noinline__ void tree_slow_call(const TreeArgs& A, const TreePlace& P, size_t node_at, int node, int head,
+                                            int start, int cnt, int n_ring, int v0, int v1, float* m, float* l,
+                                            float (&o)[4]) {
+  tree_slow_row<I8>(A, P, node_at, node, head, start, cnt, n_ring, v0, v1, m, l, o);
+}
+
 // Grid (tiles of 128 rows * kvh * nsplit, sessions).
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __grid_constant__ TreeArgs A, int* werr) {
@@ -926,7 +935,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
       if (hh >= 0) ll = max(ll, hh - A.slots + 1);
       const int c2 = ll <= hh ? hh - ll + 1 : 0, s2 = c2 ? (int)((long)(ll - base) % A.slots) : 0;
       float m2 = -INFINITY, l2 = 0.f, o2[4] = {0.f, 0.f, 0.f, 0.f};
-      tree_slow_row<I8>(A, P, at2, n2, h2, s2, c2, n_ring, blk0 * BN, min((blk0 + nblk) * BN, P.total), &m2, &l2, o2);
+      tree_slow_call<I8>(A, P, at2, n2, h2, s2, c2, n_ring, blk0 * BN, min((blk0 + nblk) * BN, P.total), &m2, &l2, o2);
       float* dst = A.nsplit > 1 ? A.part + ((((size_t)b * A.kvh + kh) * A.nsplit + z) * R + q2) * (A.vh + 2)
                                 : A.out + (at2 * A.heads + h2) * A.vh;
       for (int j = 0; j < 4; ++j)
