@@ -230,6 +230,28 @@ def test_keys_at_the_top_of_the_range(cuda, int8):
 
 
 @pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("T,heads,kvh,qk,vh,slots", [(3, 12, 2, 48, 64, 90), (20, 12, 2, 48, 64, 90), (9, 16, 2, 128, 128, 200),
+                                                     (24, 4, 1, 64, 64, 4200), (2, 6, 1, 48, 64, 9000)])
+def test_padding_nodes_with_queries_that_are_no_numbers(cuda, int8, T, heads, kvh, qk, vh, slots):
+    """Nodes whose queries hold NaN get NaN, or zeros where they see nothing; the
+    others are as they would be without them."""
+    torch = cuda
+    c = Tree(2, T, heads, kvh, qk, vh, slots, slots - 5, int8, seed=T)
+    blind, seeing = T - 1, 1                            # the last sees nothing at all
+    c.mask[:, blind] = 0
+    c.hi[:, blind] = -1
+    want, tol = c.want()
+    c.q[:, blind, 3] = c.q[:, seeing, ::7] = np.nan
+    got = c.run(torch).cpu().numpy()
+    others = [t for t in range(T) if t not in (blind, seeing)]
+    assert np.all(np.abs(got - want)[:, others] <= tol[:, others])
+    first = (np.arange(0, c.ldq, 7)[:, None] // qk == np.arange(heads)).any(0)   # heads with a NaN
+    if blind != seeing:
+        assert np.isnan(got[:, seeing][:, first]).all()
+    assert np.all(got[:, blind] == 0.0)
+
+
+@pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("T,heads,kvh,qk,vh,slots", [(65, 4, 1, 48, 64, 300), (40, 8, 2, 64, 64, 90), (33, 8, 2, 128, 128, 200),
                                                      (70, 2, 1, 128, 128, 4200), (150, 1, 1, 48, 64, 5000)])
 def test_every_row_done_again(cuda, int8, T, heads, kvh, qk, vh, slots):
