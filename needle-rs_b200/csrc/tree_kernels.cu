@@ -658,11 +658,20 @@ again:
     __syncwarp();  // this buffer is refilled next
   }
   cp_wait<0>();
+  bool lost = false;  // a row whose sum is no number
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) {
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+    lost |= !(sum[i] <= 3.4028234e38f);
+  }
   // A weight of zero times a value that is no number must not count (a node
   // masked for some rows only may hold anything), and neither may a scale that a
-  // row does not see cost it bits: where an output came out infinite or NaN, or
-  // the value scales lie more than 2^12 apart, the warp takes its blocks again,
-  // position by position in f32.
+  // row does not see cost it bits: where an output came out infinite or NaN (of a
+  // row whose sum is a number; the others see to themselves below), or the value
+  // scales lie more than 2^12 apart, the warp takes its blocks again, position by
+  // position in f32: 256 sessions over 1043 int8 positions 49 -> 190 us with one such
+  // value scale in each.
   if (!careful) {
     bool odd = I8 && vexp - vlow > 12;
 #pragma unroll
@@ -670,7 +679,8 @@ again:
 #pragma unroll
       for (int n = 0; n < VN; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= !(fabsf(o[m][n][e]) <= 3.4028234e38f);
+        for (int e = 0; e < 4; ++e)
+          odd |= !(fabsf(o[m][n][e]) <= 3.4028234e38f) && sum[2 * m + (e >> 1)] <= 3.4028234e38f;
     if (__any_sync(0xffffffffu, odd)) {
       careful = true;
       __syncwarp();
@@ -684,13 +694,6 @@ again:
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int n = 0; n < VN; ++n) o[m][n][0] *= f, o[m][n][1] *= f, o[m][n][2] *= f, o[m][n][3] *= f;
-  }
-  bool lost = false;
-#pragma unroll
-  for (int i = 0; i < 2 * MT; ++i) {
-    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-    lost |= !(sum[i] <= 3.4028234e38f);
   }
   // ---- the four warps' results meet (shared memory reused)
   __syncthreads();
