@@ -26,6 +26,10 @@ struct TreeArgs {
   float* part;             // [B][kvh][nsplit][T * rep][vh + 2] when nsplit > 1
 };
 
+// A product of a scaled query and codes is up to 2^28: times a key scale above this
+// it could pass the range before the query's power of two is taken back.
+constexpr float KEY_SCALE_FAR = 0x1p96f;
+
 // 2^x, relative error about 2^-22; arguments here are <= 0.
 __device__ __forceinline__ float ex2(float x) {
   float y;

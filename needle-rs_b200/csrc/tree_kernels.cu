@@ -151,13 +151,13 @@ __device__ __forceinline__ void tree_copy(char* buf, const char* k, const char* 
 }
 
 // A warp's rows again, over its own blocks of PB positions and in plain f32: those
-// whose sum is no number, or all of them, of the TILE rows of `mine` (row stride
-// PW: outputs, then max and sum at AT). Everything is worked out afresh, so that
+// of the TILE rows of `mine` (row stride PW: outputs, then max and sum at AT) whose
+// sum is no number or, with `far`, that see a key scale above KEY_SCALE_FAR. Everything is worked out afresh, so that
 // the kernel keeps no register for it (with the ranges handed over the 128-wide
 // forms were 5 to 7 % slower; so, f32 ones are 3 %: 32 x 1043 with 6 rows 218 -> 225
 // us, int8 50.1 -> 49.9).
 template <bool I8, int TILE, int PB, int PW, int AT>
-__device__ __noinline__ void tree_again(const TreeArgs& A, float* mine, bool all) {
+__device__ __noinline__ void tree_again(const TreeArgs& A, float* mine, bool far) {
   const int b = blockIdx.y, wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int z = blockIdx.x % A.nsplit, kh = blockIdx.x / A.nsplit % A.kvh, tile = blockIdx.x / A.nsplit / A.kvh;
   const int R = A.T * A.rep, r0 = tile * TILE, rows = min(TILE, R - r0);
@@ -177,7 +177,8 @@ __device__ __noinline__ void tree_again(const TreeArgs& A, float* mine, bool all
   P.drafted = A.drafted, P.slot0 = base % A.slots, P.slots = A.slots, P.kvh = A.kvh, P.total = A.drafted + n_ring;
   for (int r = 0; r < rows; ++r) {
     float* row = mine + (size_t)r * PW;
-    if (!all && row[AT + 1] <= 3.4028234e38f) continue;
+    const bool number = row[AT + 1] <= 3.4028234e38f;
+    if (!far && number) continue;
     const int rr = r0 + r, node = A.by_rep.div(rr), head = kh * A.rep + rr - node * A.rep;
     const size_t node_at = (size_t)b * A.T + node;
     const float* q = A.q + node_at * A.ldq + (size_t)head * A.qk;
@@ -188,6 +189,19 @@ __device__ __noinline__ void tree_again(const TreeArgs& A, float* mine, bool all
     int l = max(A.lo[node_at], 0);
     if (h >= 0) l = max(l, h - A.slots + 1);
     const int cnt = l <= h ? h - l + 1 : 0, start = cnt ? (int)((long)(l - base) % A.slots) : 0;
+    if (number) {  // whether the row sees one of the scales at all
+      bool sees = false;
+      for (int blk = blk0; blk < blk1; blk += TREE_WARPS) {
+        const int v0 = blk < ring_blocks ? P.drafted + blk * PB : (blk - ring_blocks) * PB;
+        const int v1 = min(v0 + PB, blk < ring_blocks ? P.total : P.drafted);
+        for (int at = v0 & ~31; at < v1; at += 32) {
+          const int v = at + lane;
+          if (v >= v0 && v < v1 && ((tree_sees(A, node_at, node, start, cnt, n_ring, at) >> lane) & 1))
+            sees |= fabsf((P.in_draft(v) ? A.tks : A.ks)[P.row(v)]) > KEY_SCALE_FAR;
+        }
+      }
+      if (!__any_sync(0xffffffffu, sees)) continue;
+    }
     float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int blk = blk0; blk < blk1; blk += TREE_WARPS) {
       const int v0 = blk < ring_blocks ? P.drafted + blk * PB : (blk - ring_blocks) * PB;
@@ -530,7 +544,7 @@ again:
     float grow = 1.f;
     float2 v2[NT];
     if (I8) {
-      if (fabsf(sc[lane]) > 0x1p96f) range[2] = 1;  // times a product of up to 2^28
+      if (fabsf(sc[lane]) > KEY_SCALE_FAR) range[2] = 1;
       const uint32_t a = __float_as_uint(fabsf(sc[PB + lane]));
       const uint32_t top = __reduce_max_sync(0xffffffffu, a);
       vlow = min(vlow, (int)(__reduce_min_sync(0xffffffffu, a ? a : 0x7f800000u) >> 23));
@@ -710,7 +724,7 @@ again:
   }
   // Rows whose sum is no number (an infinite key has no finite parts: its
   // remainder is NaN, but its score may be -inf and weigh nothing) are done again,
-  // and so is every row where a score may have passed the range before the query's
+  // and so are rows of which a score may have passed the range before the query's
   // power of two is taken back.
   const bool far = I8 && *(volatile int*)(range + 2);
   if (__builtin_expect(__any_sync(0xffffffffu, lost || far), 0)) {

@@ -657,8 +657,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + 1) ^ (kp & 7)) << 4)) =
                   make_uint4(w[4], w[5], w[6], w[7]);
             }
-            // A product of the scaled query is up to 2^28: key scales from 2^96 on could take it past the range.
-            sane[h] = fabsf(ksc[h]) <= 0x1p96f && fabsf(vsc[h]) <= 3.4028234e38f;
+            sane[h] = fabsf(ksc[h]) <= KEY_SCALE_FAR && fabsf(vsc[h]) <= 3.4028234e38f;
           }
           // Value scales, held so that the largest so far is in [2^13, 2^14).
           uint32_t top = 0, least = 0x7f800000u;
@@ -721,7 +720,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) tree_umma_kernel(const __
               *reinterpret_cast<uint4*>(at + C::K_TILE) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
             }
             if (lane % LK == 0) col_k[st * BN + kp] = v0 + kp < P.total ? __uint_as_float((uint32_t)(ef - 13) << 23) : 0.f;
-            if (!(mx <= 0x1p96f)) outs |= 1u << (kp & 31);  // as for int8: scaled products are up to 2^35
+            if (!(mx <= KEY_SCALE_FAR)) outs |= 1u << (kp & 31);  // the scale is 2^13 to 2^14 times less, a product up to 2^35
           }
           outs = __reduce_or_sync(0xffffffffu, outs);
           if (lane == 0) odd[st * 2 * NC + kw] = outs;
