@@ -116,9 +116,10 @@ __device__ __forceinline__ float block_max(float v, float* red) {
 // the vector's end hold 0): scale = absmax / 127 (1 for an all-zero vector),
 // code = clamp(roundf(x * (1 / scale)), -128, 127). IEEE division for the
 // scale and its reciprocal and roundf's half-away-from-zero rounding make it
-// bit-exact with the reference on identical inputs. This is the only int8
-// quantiser on the GPU: the KV append and the query fake-quant of qkv_post and
-// the standalone nd_kv_quant all call it. Returns the scale; the codes come
+// bit-exact with the reference on identical inputs. The engine's KV append, the
+// query fake-quant of qkv_post and the standalone nd_kv_quant all call it;
+// nd_kv_append (code_of, kv_kernels.cu) has the same rule in fewer instructions,
+// tested against this one to the bit. Returns the scale; the codes come
 // back as floats holding integers in [-128, 127]. Split in two steps
 // (kv_quant_absmax_warp, kv_quant_codes) so that a warp holding several
 // vectors can run their reductions back to back.

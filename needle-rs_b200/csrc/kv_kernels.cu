@@ -75,8 +75,10 @@ __device__ __forceinline__ int code_of(float x, float inv) {
 // places of `rows` rows once (shared memory); its groups of lanes then take the
 // rows' vectors (row, key or value, head), KV_VECS of them loaded before the
 // first is quantised. A row's vectors are neighbours, so a warp reads whole
-// cache lines of a projection row. 4 bytes read and 1 written per value; at
-// serving sizes the quantiser's instructions bound it, not the bytes.
+// cache lines of a projection row. 4 bytes read and 1 written per value: 16384 rows
+// of 224 values are 2.8 us of bytes and take 10.4. A block makes one pass, and its
+// warps wait at its one barrier for the places (4.2 barrier stalls per issue
+// against 0.4 on memory, 63 % of the issue slots busy).
 constexpr int KV_VECS = 4;
 
 template <bool VEC, int L, int S>
@@ -291,8 +293,9 @@ bool vec_ok(const void* p, int align) { return ((uintptr_t)p) % align == 0; }
 
 // Rows a block of kv_rows_kernel moves: KV_FLIGHT pieces a thread, fewer where that
 // would leave SMs without a block. 133504 int8 rows read back (224 values): 4 rows
-// a block 72 us, 8: 52, 16: 37, 32 (the rule): 31.0 (5.0 TB/s of 6.6 for a copy),
-// 64: 31.1. f32 rows, 16384 written and read: 4: 31, 8: 21, 16: 18.6, 32: 16.3.
+// a block 72 us, 8: 51, 16: 37, 32: 30.9, 36 (the rule): 30.8 (5.0 TB/s of 6.6 for a
+// copy), 64: 30.9. f32 rows, 16384 written and read: 4: 31, 8: 21, 16: 18.4, 32: 16.1,
+// 36 (the rule): 16.5, of which the write takes 8.3 (4.5 us of bytes), 64: 16.6.
 static int kv_block_rows(int M, int pieces) {
   int rows = std::max(1, std::min(KV_ROWS, KV_THREADS * KV_FLIGHT / std::max(1, pieces)));
   while (rows > 1 && (M - 1) / rows + 1 < 148) rows /= 2;
@@ -341,8 +344,8 @@ cudaError_t launch_kv_append(const float* k, int ldk, const float* v, int ldv, c
   const bool vec = qk % 4 == 0 && vh % 4 == 0 && ldk % 4 == 0 && ldv % 4 == 0 && vec_ok(k, 16) && vec_ok(v, 16) &&
                    vec_ok(kc, 4) && vec_ok(vc, 4);
   // Rows a block: KV_VECS vectors a group, fewer where SMs would be without a
-  // block. 16384 rows of 2 heads of 48 | 64, written and read back: 2 rows 39 us, 4:
-  // 26.5, 8: 22.3, 16 (the rule): 19.3, 32: 20.7, 64: 22.7; the write alone 11.2.
+  // block. 16384 rows of 2 heads of 48 | 64: 2 rows 30.9 us, 4: 18.6, 8: 12.4, 16 (the
+  // rule): 10.4, 32: 10.6, 64: 12.4.
   const int big = std::max(qk, vh), L = big <= 64 ? 16 : 32;
   int rows = std::max(1, std::min(KV_ROWS, (big > 128 ? 2 : KV_VECS) * (KV_THREADS / L) / (2 * kvh)));
   while (rows > 1 && (M - 1) / rows + 1 < 148) rows /= 2;

@@ -17,8 +17,10 @@
 // they accumulate, always towards zero: so a block's products start from zero,
 // remainders first, and are added to the running outputs (and long dot products
 // chunk by chunk) in f32. Left in the accumulators over 5651 positions the bias
-// was 8e-7 of the result against 4e-7 of the plain 32-bit form. Eight sessions'
-// single token over 512 positions take 12 us: latency, 64 blocks of a short chain.
+// was 8e-7 to 1.5e-6 of the result against 3.4e-7 of the plain 32-bit form. Eight
+// sessions' single token over 512 positions take 10.4 us (f32 14.5; nd_attend_step 20.5
+// and 22.7), with a draft of one node 12.3: latency, 64 blocks of a short chain. 256
+// sessions over 1043 positions take 47 (f32 121; nd_attend_step 66 and 206).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -910,11 +912,15 @@ int tree_tile_rows(int R, int qk, int vh) { return R <= 16 || qk > 64 || vh > 64
 // mma.sync: as many as keep the grid in one wave (clusters leave a few places
 // empty), each of at least 8 blocks of 32 positions; 9 to 16 are 8, which join
 // inside their cluster. Measured at one token, 6 rows of 48/64 int8 (splits: us):
-//   16 x 1000   2: 17.4  4: 14.0  8: 12.9      32 x 1000   2: 18.0  6: 14.8  8: 22.8
-//   64 x 1000   1: 20.9  2: 20.2  3: 18.7  4: 27.9
-//   256 x 1000  1: 44.3  2: 56.9               16 x 4000   8: 18.7  9: 22.9  16: 27.0
-//   1 x 6000    4: 28.9  8: 19.8  16: 18.7  24: 16.7
+//   16 x 1000   2: 17.4  4: 14.3  8: 13.0      32 x 1000   2: 18.1  6: 15.4  8: 22.9
+//   64 x 1000   1: 22.1  2: 20.3  3: 18.8  4: 28.2
+//   256 x 1000  1: 45.2  2: 58.1               16 x 4000   8: 18.8  9: 22.9  16: 27.2
+//   1 x 6000    4: 29.0  8: 20.8  16: 18.8  24: 16.7
 // and with eight splits left to a join kernel 16 x 1000 takes 15.3, 16 x 4000 20.8.
+// Both forms plan from `slots`, as the ranges lie on the device: a ring much larger
+// than what is seen of it is split as if full. Eight sessions that see 512
+// positions take 17.9 us in rings of 33000 places against 14.5 in rings of 544 (12 rows
+// of a KV head; 96 rows, tcgen05: 23.5 against 20.5).
 TreePlan tree_plan(const void* k, const void* v, const void* tk, const void* tv, const float* out, int int8, int B,
                    int T, int heads, int kvh, int qk, int vh, int slots) {
   const int es = int8 ? 1 : 4, R = T * (heads / kvh);

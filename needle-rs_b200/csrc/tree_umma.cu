@@ -31,7 +31,7 @@
 //
 // Measured: 256 sessions x 96 rows x 1043 int8 positions (48/64) 77 us (0.9 TB/s,
 // 20 % of the tensor pipe); 16 x 288 rows x 2051 f32 positions 65 us; 4 x 8 heads x
-// 128 rows x 32771 int8 positions (128 wide) 219 us (1.1 TB/s, 28 %). The chain of a
+// 128 rows x 32771 int8 positions (128 wide) 220 to 228 us (1.1 TB/s, 28 %). The chain of a
 // softmax step bounds the int8 forms: about 2900 cycles alone, 4300 with two blocks
 // on the SM, no pipe above 40 %.
 //
@@ -990,11 +990,14 @@ typedef TreeUmma<false, 8, 128, 2, 2> UmmaF32x128;
 // More than 16 rows, whole 16-byte pieces and MMA steps. A step costs nearly the
 // same for 17 rows as for 128; mma.sync pays per 16 rows. Measured, mma.sync -> here:
 //   rows   48/64 int8, 256 x 1043   48/64 f32, 128 x 1043   128 int8, 4 x 16000   128 f32, 32 x 1043
-//    12        53 ->  62 us              66 ->  68 us            89 -> 128 us         226 -> 189 us
-//    24        72 ->  63                 84 ->  69              155 -> 130            424 -> 188
-//    48       135 ->  75                156 ->  72              268 -> 133            627 -> 190
-//    96       204 ->  78                228 ->  75              522 -> 137           1159 -> 198
-// and at eight sessions of 1043 (48/64 int8) 12 rows 15.8 -> 17.2, 24 rows 21.6 -> 17.5.
+//     6        49 ->  62 us              64 ->  68 us            83 -> 114 us         225 -> 186 us
+//    12        53 ->  62                 66 ->  69               88 -> 115            231 -> 186
+//    24        72 ->  63                 84 ->  69              155 -> 116            438 -> 187
+//    48       136 ->  74                156 ->  72              270 -> 119            646 -> 190
+//    96       205 ->  78                228 ->  76              527 -> 124           1193 -> 194
+// and at eight sessions of 1043 (48/64 int8) 6 rows 12.6 -> 16.8, 12: 15.4 -> 16.7, 24:
+// 22.1 -> 17.1. One bound for all forms: of 128-wide f32 heads it lies too high, and up
+// to 16 rows there take the slower form.
 bool tree_umma_takes(int int8, int rows, int qk, int vh, int piece) {
   return piece == 16 && qk % 16 == 0 && vh % 16 == 0 && rows > 16;
 }
