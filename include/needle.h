@@ -384,9 +384,9 @@ int nd_logits_adjust(const float *logits, int ld, int rows, int vocab, float *ou
 /* Waits that gave up. The tcgen05 kernels (nd_cq_project and
  * nd_cq_project_grouped on path 3, which path 0 takes for M > 8; nd_attend_tree
  * with more than 16 rows of a KV head) wait inside a block, each wait bounded to
- * about a second. Should one give up, its kernel raises a flag of the current device and
- * its outputs are not to be used (nd_attend_tree writes NaN to the rows
- * concerned); the call that launched it has returned 0 by then.
+ * about a second. Should one give up, its kernel raises a flag of the current
+ * device and its outputs are not to be used (nd_attend_tree writes NaN to the
+ * rows concerned); the call that launched it has returned 0 by then.
  * nd_take_wait_error reads the flag into *gave_up (1: raised since it was last
  * taken) and clears it; call it after synchronising with the streams of the
  * calls in question, not during a capture. nd_wait_flag gives the flag's device
