@@ -101,9 +101,9 @@ __device__ __forceinline__ uint32_t tree_sees(const TreeArgs& A, size_t node_at,
 // rows whose keys, values or scales split operands cannot hold. Adds them to the
 // row's running log2 max, sum, and dims lane + 32 j of the output.
 template <bool I8>
-__device__ __forceinline__ void tree_slow_row(const TreeArgs& A, const TreePlace& P, size_t node_at, int node, int head,
-                                           int start, int cnt, int n_ring, int v0, int v1, float* m_run, float* l_run,
-                                           float (&o)[4]) {
+__device__ __forceinline__ void tree_slow_row(const TreeArgs& A, const TreePlace& P, size_t node_at, int node,
+                                              int head, int start, int cnt, int n_ring, int v0, int v1, float* m_run,
+                                              float* l_run, float (&o)[4]) {
   const int lane = threadIdx.x & 31;
   const float* q = A.q + node_at * A.ldq + (size_t)head * A.qk;
   float m = *m_run, l = *l_run;

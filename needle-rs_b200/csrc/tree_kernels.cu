@@ -154,10 +154,11 @@ __device__ __forceinline__ void tree_copy(char* buf, const char* k, const char* 
 
 // A warp's rows again, over its own blocks of PB positions and in plain f32: those
 // of the TILE rows of `mine` (row stride PW: outputs, then max and sum at AT) whose
-// sum is no number or, with `far`, that see a key scale above KEY_SCALE_FAR. Everything is worked out afresh, so that
-// the kernel keeps no register for it (with the ranges handed over the 128-wide
-// forms were 5 to 7 % slower; so, f32 ones are 3 %: 32 x 1043 with 6 rows 218 -> 225
-// us, int8 50.1 -> 49.9).
+// sum is no number or, with `far`, that see a key scale above KEY_SCALE_FAR.
+// Everything is worked out afresh, so that the kernel keeps no register for it
+// (with the ranges handed over the 128-wide forms were 5 to 7 % slower than without
+// this call; as it is, f32 ones are 3 %: 32 x 1043 with 6 rows 218 -> 225 us, int8
+// 50.1 -> 49.9).
 template <bool I8, int TILE, int PB, int PW, int AT>
 __device__ __noinline__ void tree_again(const TreeArgs& A, float* mine, bool far) {
   const int b = blockIdx.y, wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -224,7 +225,8 @@ __device__ __noinline__ void tree_again(const TreeArgs& A, float* mine, bool far
 // the ring's (offsets 0 .. n_ring - 1 from the tile's lowest position) and
 // then the draft's nodes.
 template <bool I8, int QKP, int VHP, int MT>
-__global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const __grid_constant__ TreeArgs A, int piece, int cluster) {
+__global__ void __launch_bounds__(TREE_THREADS) attend_tree_kernel(const __grid_constant__ TreeArgs A, int piece,
+                                                                   int cluster) {
   using TT = TreeTile<I8, QKP, VHP>;
   constexpr int PB = TT::PB, NT = PB / 8;        // 8-position score tiles of a block
   constexpr int KC = QKP / 16, VN = VHP / 8;     // 16-dim chunks of a key, 8-dim tiles of an output
